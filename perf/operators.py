@@ -168,7 +168,7 @@ def _plain_scores(s):
         dx.scatter_add_(-1, token, g)
         out["grad"] = torch.where(valid.unsqueeze(-1), dx, 0.0).to(s["logits"].dtype)
         return out
-    out["stats"] = torch.where(valid.unsqueeze(-1), torch.cat([m, log_total], -1), 0.0)
+    out["stats"] = torch.where(valid.unsqueeze(-1), torch.cat([m, total], -1), 0.0)
     # alternatives: one whole number a token that orders by value, then by lowest index
     bits = x.contiguous().view(torch.int32).long()
     order = torch.where(bits < 0, -(bits & 0x7FFFFFFF), bits)
@@ -282,7 +282,7 @@ def _exact_rows(case, s, rows):
             out["grad"] = dx * keep[:, None]
             return out
         m = x.max(-1).values
-        out["stats"] = torch.stack([m * keep, (torch.logsumexp(x, -1) - m) * keep], -1)
+        out["stats"] = torch.stack([m * keep, (torch.logsumexp(x, -1) - m).exp() * keep], -1)
         ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :case["top"]]
         top = logp_all[line[:, None], ids]
         none = ~keep[:, None] | torch.isinf(top)
