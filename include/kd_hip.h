@@ -327,6 +327,83 @@ int kd_batch_raw_lattice_copy(kd_batch *b, const int64_t *state_off, const int64
  * bit; with the switch off nothing changes. */
 int kd_batch_set_log_softmax(kd_batch *b, int32_t on);
 
+/* ---- scores of given tokens, alternatives, distillation: operators over rows of logits -------
+ * The reference ends where its decoders return symbols; how sure the model was of them, what else
+ * a frame could have been, and how one model's frames differ from another's (a smaller or a
+ * quantised one's, and the gradient that trains it) is left to the caller.  These entries compute
+ * that on the rows the search reads, on the GPU.
+ *
+ * Rows: [batch][steps][vocab] logits (unit stride over the vocabulary, any non-negative strides,
+ * in elements, over the others; 2-D logits are batch = 1).  `lengths` (device, [batch], or NULL):
+ * rows at or behind their utterance's length are not read, their outputs are 0 (alternatives
+ * -1 / -inf) and so are their gradients.  Arrays of one value a row are contiguous [batch][steps].
+ *
+ * All pointers are device pointers on `device`.  A call enqueues on `stream` (a hipStream_t, NULL =
+ * default) and returns: no allocation, no synchronisation, no state of the library's, so calls may
+ * be captured into a graph and made from several threads.  The workspace is the caller's, 16-byte
+ * aligned, and in use until the call's work on the stream is done: calls that may overlap (another
+ * stream, another captured graph) need one each.  Sums and statistics are f32; results do not
+ * depend on how rows are dealt out and are the same from run to run.
+ * vocab <= 2^24; at most 2^24 - 1 rows (x ceil(row bytes / 32 KiB) where a row is longer than that;
+ * four times as many rows of up to 8 KiB). */
+#define KD_DTYPE_F32 0
+#define KD_DTYPE_F16 1
+#define KD_DTYPE_BF16 2
+typedef struct kd_frame_rows {
+  const void *logits;
+  int64_t batch, steps, vocab;
+  int64_t batch_stride, row_stride; /* elements */
+  const int32_t *lengths;           /* device, [batch], or NULL */
+  int32_t dtype;                    /* KD_DTYPE_*: of the logits and of their gradient */
+  int32_t device;
+} kd_frame_rows;
+
+/* Per row x: m = max x, s = sum exp(x_j - m), log p_j = x_j - m - log s, and
+ *   logp[row]     log p of the row's token (`tokens`: int32 or int64 as token_bytes says, [rows], or
+ *                 NULL; a token outside [0, vocab) gives 0)
+ *   entropy[row]  -sum_j p_j log p_j
+ *   stats[row][2] m, s (what the gradient needs)
+ *   top_ids, top_logp [rows][top]  the `top` <= 64 largest logits' columns and log p, in falling
+ *                 order, the lowest column first among equals.  A logit of -inf is no alternative:
+ *                 places without one hold -1 / -inf.
+ * A row of -inf alone: logp -inf, entropy 0, stats -inf / 0, no alternatives.  A row with NaN or
+ * +inf: logp, entropy and top_logp NaN, top_ids -1. */
+size_t kd_token_scores_workspace(const kd_frame_rows *rows, int32_t top);
+int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token_bytes, int32_t top,
+                    float *logp, float *entropy, float *stats, float *top_logp, int32_t *top_ids,
+                    void *workspace, size_t workspace_bytes, void *stream);
+/* The logits' gradient for upstream gradients of logp and entropy ([rows], either may be NULL: 0):
+ *   grad_j = grad_logp ([j = token] - p_j) - grad_entropy p_j (log p_j + entropy)
+ * into `grad` (the logits' dtype and shape, strides of its own; rows must not overlap).  A row of
+ * -inf alone gets zeros. */
+int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t token_bytes,
+                         const float *stats, const float *entropy, const float *grad_logp,
+                         const float *grad_entropy, void *grad, int64_t grad_batch_stride,
+                         int64_t grad_row_stride, void *stream);
+
+/* A teacher's tokens and logits (or log-probabilities: only differences count), [rows][slots],
+ * contiguous, slots <= 256; an id outside [0, vocab) marks an empty slot. */
+typedef struct kd_teacher_rows {
+  const void *ids;    /* int32 or int64 as id_bytes says */
+  const void *logits; /* KD_DTYPE_* */
+  int32_t slots, id_bytes, dtype;
+} kd_teacher_rows;
+/* Distillation: with q = softmax(teacher / temperature) over a row's filled slots and
+ * p = softmax(x / temperature) over the vocabulary,
+ *   loss[row] = weight sum_k q_k (log q_k - log p_{id_k})     (a q_k of 0 adds 0)
+ *   grad_j    = weight upstream / temperature (p_j - sum_{k: id_k = j} q_k)
+ * `weights`, `upstream`: [rows] or NULL (1).  A row of weight 0 or without a filled slot is not
+ * read: loss 0, gradient 0.  A teacher's token that the student has at -inf: loss +inf (a student
+ * row of -inf alone: p = 0).  `grad` NULL: the loss alone.  `stats` ([rows][2], or NULL with a
+ * loss): maximum and sum of the row, written with a loss; with `loss` NULL they are read, and the
+ * call computes the gradient alone (the same inputs as the call that wrote them).  Loss and
+ * gradient in one call read a row of up to 32 KiB once. */
+size_t kd_distill_loss_workspace(const kd_frame_rows *rows);
+int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, const float *weights,
+                    float temperature, float *loss, float *stats, const float *upstream, void *grad,
+                    int64_t grad_batch_stride, int64_t grad_row_stride, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 /* ---- exported results in DEVICE memory ---------------------------------------------
  * The kernel writes exported lattices into a pinned host pool of the batch.  A caller that
  * wants them on the GPU as well -- the multi-GPU gather hands RCCL a device buffer: no host

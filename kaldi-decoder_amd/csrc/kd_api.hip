@@ -31,6 +31,15 @@ int Fail(int code, const std::string &msg) {
   return code;
 }
 
+}  // namespace
+
+namespace kd {
+// (kd_frames.hip reports through the same thread-local message)
+int SetError(int code, const std::string &msg) { return Fail(code, msg); }
+}  // namespace kd
+
+namespace {
+
 #define KD_HIP_TRY(expr)                                                            \
   do {                                                                              \
     hipError_t e_ = (expr);                                                         \

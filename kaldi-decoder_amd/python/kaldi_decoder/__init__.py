@@ -8,7 +8,9 @@ decoder.  There is no CPU fallback: importing without the built extension, or
 decoding without a GPU, raises.
 
 Submodules: `cabi` (ctypes binding of the C ABI), `synth` (seeded synthetic
-graphs and log-probs), `sharded` (multi-GPU split / gather helpers).
+graphs and log-probs), `sharded` (multi-GPU split / gather helpers), `scoring` (token
+post-processing, WER), `frames` (scores of tokens, alternatives and distillation over
+rows of logits on the GPU).
 """
 import os as _os
 

@@ -39,6 +39,8 @@ SYMBOLS = (
     "kd_batch_create_simple", "kd_batch_decode_async", "kd_batch_decode", "kd_batch_capacity",
     "kd_batch_set_output_buffer", "kd_batch_raw_lattice_table", "kd_batch_set_log_softmax",
     "kd_batch_split_info", "kd_batch_set_split", "kd_batch_sched_profile", "kd_batch_set_lazy_prune",
+    "kd_token_scores_workspace", "kd_token_scores", "kd_token_scores_grad",
+    "kd_distill_loss_workspace", "kd_distill_loss",
 )
 SPLIT_NAMES = ("split", "large_cus", "large_workgroups", "small_workgroups", "mig_lo", "mig_hi",
                "prune_small", "min_batch")
@@ -57,6 +59,19 @@ class LatticeOptions(C.Structure):
                 ("beam_delta", C.c_float), ("hash_ratio", C.c_float), ("prune_scale", C.c_float),
                 ("arena_tokens", C.c_int64), ("arena_links", C.c_int64),
                 ("table_slots", C.c_int32), ("max_frames", C.c_int32), ("no_grow", C.c_int32)]
+
+
+class FrameRows(C.Structure):
+    """kd_frame_rows: rows of logits on a device."""
+    _fields_ = [("logits", C.c_void_p), ("batch", C.c_int64), ("steps", C.c_int64), ("vocab", C.c_int64),
+                ("batch_stride", C.c_int64), ("row_stride", C.c_int64), ("lengths", C.c_void_p),
+                ("dtype", C.c_int32), ("device", C.c_int32)]
+
+
+class TeacherRows(C.Structure):
+    """kd_teacher_rows: the tokens a teacher lists, and their logits."""
+    _fields_ = [("ids", C.c_void_p), ("logits", C.c_void_p), ("slots", C.c_int32), ("id_bytes", C.c_int32),
+                ("dtype", C.c_int32)]
 
 
 _i32p = np.ctypeslib.ndpointer(np.int32, flags="C_CONTIGUOUS")
@@ -143,6 +158,15 @@ def lib():
     L.kd_batch_set_log_softmax.argtypes = [C.c_void_p, C.c_int32]
     L.kd_batch_raw_lattice_table.argtypes = [C.c_void_p, C.POINTER(C.c_int64),
                                              np.ctypeslib.ndpointer(np.int64, flags="C_CONTIGUOUS")]
+    rows, ptr = C.POINTER(FrameRows), C.c_void_p
+    L.kd_token_scores_workspace.argtypes = [rows, C.c_int32]
+    L.kd_token_scores_workspace.restype = C.c_size_t
+    L.kd_token_scores.argtypes = [rows, ptr, C.c_int32, C.c_int32, ptr, ptr, ptr, ptr, ptr, ptr, C.c_size_t, ptr]
+    L.kd_token_scores_grad.argtypes = [rows, ptr, C.c_int32, ptr, ptr, ptr, ptr, ptr, C.c_int64, C.c_int64, ptr]
+    L.kd_distill_loss_workspace.argtypes = [rows]
+    L.kd_distill_loss_workspace.restype = C.c_size_t
+    L.kd_distill_loss.argtypes = [rows, C.POINTER(TeacherRows), ptr, C.c_float, ptr, ptr, ptr, ptr, C.c_int64,
+                                  C.c_int64, ptr, C.c_size_t, ptr]
     _lib = L
     return L
 
@@ -440,6 +464,27 @@ class Batch:
                             gc[a:b].copy(), ac[a:b].copy(),
                             (float(fw[2 * i]), float(fw[2 * i + 1]))))
         return out
+
+    def best_path_scores(self, logits, lengths=None, top=0, use_final_probs=True):
+        """How sure the model was of what the decode returned: (paths, tokens, scores).  `logits`
+        [B, T, V]: the rows that were decoded, one matrix an utterance as in decode_tensor, or the
+        logits they are the log_softmax of (any type frames.token_scores takes).  `tokens` int32 [B, T]:
+        the column that each frame of the best path took -- LogLikelihood(frame, ilabel) reads column
+        ilabel - 1 (csrc/decodable-ctc.cc:22-31) --, -1 behind its end; `scores`: frames.TokenScores of
+        them, with `top` alternatives a frame."""
+        import torch
+        from . import frames
+        if logits.dim() != 3 or logits.shape[0] != self.batch:
+            raise ValueError("best_path_scores needs the logits [B, T, V] of the utterances decoded")
+        paths = self.best_paths(use_final_probs)
+        tokens = np.full(logits.shape[:2], -1, np.int32)
+        for i, path in enumerate(paths):
+            labels = path.isyms
+            if len(labels) > logits.shape[1]:
+                raise ValueError(f"utterance {i}: a best path of {len(labels)} frames, logits of {logits.shape[1]}")
+            tokens[i, :len(labels)] = labels - 1
+        tokens = torch.from_numpy(tokens).to(logits.device)
+        return paths, tokens, frames.token_scores(logits, tokens, top=top, lengths=lengths)
 
     def frame_tokens(self, utt, frame_plus_one):
         cnt = C.c_int32(0)
