@@ -374,8 +374,8 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
                     void *workspace, size_t workspace_bytes, void *stream);
 /* The logits' gradient for upstream gradients of logp and entropy ([rows], either may be NULL: 0):
  *   grad_j = grad_logp ([j = token] - p_j) - grad_entropy p_j (log p_j + entropy)
- * into `grad` (the logits' dtype and shape, strides of its own; rows must not overlap).  A row of
- * -inf alone gets zeros. */
+ * into `grad` (the logits' dtype and shape, strides of its own; rows must not overlap; the logits
+ * themselves will do: the gradient is then written over them).  A row of -inf alone gets zeros. */
 int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t token_bytes,
                          const float *stats, const float *entropy, const float *grad_logp,
                          const float *grad_entropy, void *grad, int64_t grad_batch_stride,
@@ -396,8 +396,8 @@ typedef struct kd_teacher_rows {
  * read: loss 0, gradient 0.  A teacher's token that the student has at -inf: loss +inf (a student
  * row of -inf alone: p = 0).  `grad` NULL: the loss alone.  `stats` ([rows][2], or NULL with a
  * loss): maximum and sum of the row, written with a loss; with `loss` NULL they are read, and the
- * call computes the gradient alone (the same inputs as the call that wrote them).  Loss and
- * gradient in one call read a row of up to 32 KiB once. */
+ * call computes the gradient alone (the same inputs as the call that wrote them).  `grad` may be
+ * the logits themselves, as in kd_token_scores_grad.  Loss and gradient in one call read a row of up to 32 KiB once. */
 size_t kd_distill_loss_workspace(const kd_frame_rows *rows);
 int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, const float *weights,
                     float temperature, float *loss, float *stats, const float *upstream, void *grad,

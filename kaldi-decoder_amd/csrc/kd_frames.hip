@@ -947,6 +947,7 @@ __global__ __launch_bounds__(kBlock) void DistillGradKernel(const DistillArgs a)
   for (int i = 0; i < Slots<TPU>::kN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
   const float m = a.stats[2 * static_cast<size_t>(u.row)], s0 = a.stats[2 * static_cast<size_t>(u.row) + 1];
   const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
+  UnitSync<TPU>();  // (the gradient may be written over the logits: every lane has its slots' first)
   WriteDistillGrad<T, NCH, TPU>(a, u, r, t, xs, list, m, s0, coef, tid);
 }
 

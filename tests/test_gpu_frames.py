@@ -201,7 +201,7 @@ def test_strides_of_the_gradient(frames):
                      lambda: torch.full((3, 9, v), 9.0).cuda()[:, :8:2]):
             out = make()
             got = frames.token_scores_grad(x, sc, tokens, None, up, up, out=out)
-            assert got is out and torch.equal(out, want)
+            assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
             base = out._base
             out.fill_(9.0)
             assert base.eq(9.0).all()  # (nothing around it was written)
@@ -274,6 +274,24 @@ def test_distillation(frames, dtype, tdtype, v, k, t):
             tol_g = tol_g + half_step(dt) * (gr.abs() + tol_g) + (2.0 ** -25 if dt == torch.float16 else 0)
             off = (got[r].double() - gr).abs()
             assert (off <= tol_g).all(), (r, off.max(), (off - tol_g).argmax())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("v", [64, 500, 5000, 9000, 16385, 70000])
+def test_gradient_over_the_logits(frames, dtype, v):
+    """`out` = the logits: the slots' logits are read before any lane writes."""
+    x = (torch.randn(40, v) * 3).to(DTYPES[dtype]).cuda()
+    ids = torch.stack([torch.randperm(v)[:64] for _ in range(40)]).cuda()
+    u, tokens, up = torch.randn(40, 64).cuda(), ids[:, 0].contiguous(), torch.randn(40).cuda()
+    loss, want = frames.distill_loss_and_grad(x, ids, u)
+    mine = x.clone()
+    loss2, got = frames.distill_loss_and_grad(mine, ids, u, out=mine)
+    assert got.data_ptr() == mine.data_ptr() and torch.equal(mine, want) and torch.equal(loss, loss2)
+    sc = frames.token_scores(x, tokens)
+    want = frames.token_scores_grad(x, sc, tokens, None, up, up)
+    mine = x.clone()
+    frames.token_scores_grad(mine, sc, tokens, None, up, up, out=mine)
+    assert torch.equal(mine, want)
 
 
 def test_gradients_against_differences(frames):
