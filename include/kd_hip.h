@@ -388,7 +388,7 @@ typedef struct kd_teacher_rows {
   const void *logits; /* KD_DTYPE_* */
   int32_t slots, id_bytes, dtype;
 } kd_teacher_rows;
-/* Distillation: with q = softmax(teacher / temperature) over a row's filled slots and
+/* Distillation: with 1e-6 <= temperature <= 1e6, q = softmax(teacher / temperature) over a row's filled slots and
  * p = softmax(x / temperature) over the vocabulary,
  *   loss[row] = weight sum_k q_k (log q_k - log p_{id_k})     (a q_k of 0 adds 0)
  *   grad_j    = weight upstream / temperature (p_j - sum_{k: id_k = j} q_k)

@@ -31,9 +31,9 @@ constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / 64;
 constexpr int kMaxTop = 64;       // alternatives a row
 constexpr int kMaxSlots = 256;    // teacher's tokens a row
-constexpr int kCap = 256;         // candidates a unit ranks (>= kMaxTop)
 constexpr int64_t kMaxVocab = int64_t(1) << 24;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
 constexpr float kLowest = -3.402823466e+38f;
 
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
@@ -119,39 +119,75 @@ __device__ inline const typename T::Store *RowPtr(const void *x, int64_t batch_s
   return static_cast<const typename T::Store *>(x) + u.b * batch_stride + u.t * row_stride;
 }
 
-// Lane `tid` of a unit holds columns [(c * TPU + tid) * kVec, + kVec) in r[c]: consecutive lanes
-// load consecutive 16 bytes.  (Rows need no alignment beyond their element's: the loads are marked
-// so and stay 16 bytes wide.)
+template <int TPU>
+constexpr int kThreads = TPU < kBlock ? kBlock : TPU;  // of a workgroup
+template <int TPU>
+__device__ inline int UnitLane() {
+  return TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
+}
+// Which of a workgroup's units a wave belongs to, and the unit's number.
+template <int TPU>
+__device__ inline int UnitInBlock() {
+  return TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+}
+template <int TPU>
+__device__ inline uint32_t UnitNumber() {
+  return TPU == 64 ? blockIdx.x * kWaves + UnitInBlock<TPU>() : blockIdx.x;
+}
+
+// Lane `tid` of a unit holds 16 bytes of columns from (c * TPU + tid) * kVec on in r[c]: consecutive
+// lanes load consecutive 16 bytes.  (Rows need no alignment beyond their element's: the loads are
+// marked so and stay 16 bytes wide.)  Where those 16 bytes would reach over the row's end the lane
+// holds the row's LAST 16 bytes, and the columns that are another lane's (or, further out, all of
+// them) are replaced by kFill: no load depends on a branch, so all NCH are in flight at once.
+template <class T>
+__device__ inline int FirstCol(int e, int n) {
+  return min(e, max(n - T::kVec, 0));
+}
 template <class T, int NCH, int TPU>
 __device__ inline void LoadUnit(const typename T::Store *p, int n, int tid, U4 (&r)[NCH]) {
+  if (n >= T::kVec) {
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int e = (c * TPU + tid) * T::kVec;
-    if (e + T::kVec <= n) {
-      r[c] = *reinterpret_cast<const typename T::Vec *>(p + e);
-    } else {
-      r[c] = U4{T::kFill, T::kFill, T::kFill, T::kFill};
-      if (e < n) {  // the row's end: at most kVec - 1 columns, one lane
-        for (int j = 0; j < T::kVec - 1; ++j) {
-          if (e + j >= n) break;
-          if (T::kVec == 4) {
-            const uint32_t v = __builtin_bit_cast(uint32_t, static_cast<float>(p[e + j]));
-            if (j == 0) r[c][0] = v;
-            if (j == 1) r[c][1] = v;
-            if (j == 2) r[c][2] = v;
-          } else {
-            const uint32_t v = reinterpret_cast<const uint16_t *>(p)[e + j];
-            const uint32_t old = j < 2 ? r[c][0] : j < 4 ? r[c][1] : j < 6 ? r[c][2] : r[c][3];
-            const uint32_t now = (j & 1) ? (old & 0xffffu) | v << 16 : (old & 0xffff0000u) | v;
-            if (j < 2) r[c][0] = now;
-            else if (j < 4) r[c][1] = now;
-            else if (j < 6) r[c][2] = now;
-            else r[c][3] = now;
-          }
+    for (int c = 0; c < NCH; ++c)
+      r[c] = *reinterpret_cast<const typename T::Vec *>(p + FirstCol<T>((c * TPU + tid) * T::kVec, n));
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if ((c + 1) * TPU * T::kVec <= n) continue;  // (no lane of this one reaches the end)
+      const int e = (c * TPU + tid) * T::kVec, others = e - FirstCol<T>(e, n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (T::kVec == 4) {
+          r[c][i] = i < others ? T::kFill : r[c][i];
+        } else {
+          uint32_t v = r[c][i];
+          v = 2 * i < others ? (v & 0xffff0000u) | (T::kFill & 0xffffu) : v;
+          r[c][i] = 2 * i + 1 < others ? (v & 0xffffu) | (T::kFill & 0xffff0000u) : v;
+        }
+      }
+    }
+  } else {  // a row of less than 16 bytes: all lane 0's
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) r[c] = U4{T::kFill, T::kFill, T::kFill, T::kFill};
+    if (tid == 0) {
+#pragma unroll
+      for (int j = 0; j < T::kVec - 1; ++j) {
+        if (j >= n) break;
+        if (T::kVec == 4) {
+          r[0][j] = __builtin_bit_cast(uint32_t, static_cast<float>(p[j]));
+        } else {
+          const uint32_t v = reinterpret_cast<const uint16_t *>(p)[j];
+          r[0][j >> 1] = (j & 1) ? (r[0][j >> 1] & 0xffffu) | v << 16 : (r[0][j >> 1] & 0xffff0000u) | v;
         }
       }
     }
   }
+}
+// Between two passes over a unit's registers: without it the compiler keeps the first pass's
+// conversions for the second, two (f16, bf16: four) times the registers.
+template <int NCH>
+__device__ inline void NewPass(U4 (&r)[NCH]) {
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) asm volatile("" : "+v"(r[c]));
 }
 
 // ---- reductions over a unit --------------------------------------------------------------------
@@ -178,17 +214,7 @@ __device__ inline float WaveSum(float v) {
   return WaveReduce(v, 0.0f, [](float a, float b) { return a + b; });
 }
 
-// A unit's scratch in LDS: of one wave (TPU 64, never synchronised with the others) or of the
-// whole workgroup.
-struct Scratch {
-  float red[kWaves];
-  int ired[kWaves];
-  int count;
-  float group_max[kBlock];
-  float cand_v[kCap];
-  int cand_i[kCap];
-};
-
+// A unit of one wave (TPU 64) is never synchronised with the workgroup's others.
 template <int TPU>
 __device__ inline void UnitSync() {
   if (TPU > 64) {
@@ -199,15 +225,23 @@ __device__ inline void UnitSync() {
   }
 }
 
-// (two barriers: `red` may be reused at once)
+// `red`: one float a wave, not written again before the unit's next barrier but one.
 template <int TPU>
 __device__ inline float UnitMax(float v, float *red) {
   v = WaveMax(v);
   if (TPU == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < TPU / 64; ++w) v = fmaxf(v, red[w]);
+  return v;
+}
+template <int TPU>
+__device__ inline float SumOf(const float *red) {
+  float v = red[0];
+#pragma unroll
+  for (int w = 1; w < TPU / 64; ++w) v += red[w];
   return v;
 }
 template <int TPU>
@@ -216,9 +250,7 @@ __device__ inline float UnitSum(float v, float *red) {
   if (TPU == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = (red[0] + red[1]) + (red[2] + red[3]);
-  __syncthreads();
-  return v;
+  return SumOf<TPU>(red);
 }
 // Sum over the unit of counts that every lane of a wave already agrees on.
 template <int TPU>
@@ -226,21 +258,59 @@ __device__ inline int UnitCount(int wave_count, int *red) {
   if (TPU == 64) return wave_count;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = wave_count;
   __syncthreads();
-  const int v = (red[0] + red[1]) + (red[2] + red[3]);
+  int v = 0;
+#pragma unroll
+  for (int w = 0; w < TPU / 64; ++w) v += red[w];
   __syncthreads();
   return v;
 }
 __device__ inline int Popc(uint64_t m) { return __popcll(m); }
 
+// ---- sums of exponentials ------------------------------------------------------------------------
+// e_j = exp2((x_j - m) k2) as exp2(fma(x_j, k2, -c)), c = m k2 rounded: one operation less an element
+// than the difference times k2, and as exact -- what the rounding of c adds to every exponent is
+// known (delta; at most 64) and taken out of the sums afterwards.  From |c| = 2^30 on (rows of the
+// type's lowest value) any column that differs from m at all is 2^64 times smaller: there a power
+// of two stands in for k2 that makes m k2 exact, about 2^40, and such columns' e 0.
+// (1.5e-6 <= k2 <= 1.5e6, the range of the temperature.)
+struct Exponent {
+  float k2, c, delta;
+  __device__ Exponent(float base, float k2_) {
+    const bool far = !(fabsf(base * k2_) < 0x1p30f) && base != INFINITY;
+    k2 = far ? __uint_as_float(__float_as_uint(0x1p40f / fabsf(base)) & 0x7f800000u) : k2_;
+    c = base * k2;
+    delta = fmaf(base, k2, -c);  // exponents come out larger by this much
+  }
+  __device__ float operator()(float x) const { return fmaf(x, k2, -c); }
+};
+
 // ---- the K largest -------------------------------------------------------------------------------
 // Order: larger value first, then lower column.  -inf and NaN are no candidates.
 //
-// 1. A threshold: the K-th largest of the maxima of groups of a unit's elements (64 or 256 groups,
-//    K <= 64 of them): at least K elements reach it, and of data in no particular order few more.
-// 2. The elements that reach it are collected in LDS.  Where they are more than the list holds
-//    (many equal values, or most of the large ones in few groups) the K-th element itself is found
-//    by bisection, its value bit by bit and then, among equals, its column: exactly K are left.
+// 1. A threshold: about the K-th largest of the maxima of 256 (a wave's unit: 64 or 256) groups of
+//    the unit's elements: at least K elements reach it, and of data in no particular order few more.
+// 2. The elements that reach it are collected in LDS, each wave's in a list of its own.  Where they
+//    are more than the lists hold (many equal values, or most of the large ones in few groups) the
+//    K-th element itself is found by bisection, its value bit by bit and then, among equals, its
+//    column: exactly K are left.
 // 3. Each candidate's place is the number of candidates ahead of it.
+constexpr int kCap = 128;       // candidates a wave's list holds; a unit of one wave: twice that
+constexpr int kMaxRanked = 512; // candidates a unit ranks
+
+struct Cand {
+  float v;
+  int32_t i;
+};
+template <int TPU>
+struct Scratch {
+  static constexpr int kW = TPU / 64;
+  static constexpr int kList = kW == 1 ? 2 * kCap : kCap;
+  float red[3][kW];
+  int count[kW];
+  float group_max[kW == 1 ? 1 : 64 * kW];
+  int place[kW == 1 ? 1 : kMaxRanked];
+  Cand cand[kW][kList];
+};
 
 // A whole number that orders as the value does (-0 and +0 alike).
 __device__ inline uint32_t OrderKey(float v) {
@@ -251,14 +321,15 @@ __device__ inline float KeyValue(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
-// The k-th largest of 64 * G values of a wave (1 <= k <= 64 * G).
+// A value that at least k (<= 64 * G) of a wave's 64 * G values reach, and few more than k do: the
+// upper half of the k-th largest's key, bit by bit.
 template <int G>
 __device__ inline float KthLargest(const float (&v)[G], int k) {
   uint32_t key[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) key[g] = OrderKey(v[g]);
   uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= 16; --bit) {
     const uint32_t c = t | (1u << bit);
     int n = 0;
 #pragma unroll
@@ -268,33 +339,52 @@ __device__ inline float KthLargest(const float (&v)[G], int k) {
       if (n == k) break;
     }
   }
-  // (broken off: every value from t upwards is among the k largest; t need not be one of them)
+  // (a key below that of -inf is a NaN's; SelectTop takes either for "all")
   return KeyValue(t);
 }
+// The same of a unit's group maxima: a lane's own in a unit of one wave, else those in LDS.
+template <int TPU>
+__device__ inline float GroupThreshold(const float (&gm)[4], const Scratch<TPU> &s, int k) {
+  if (TPU == 64) {
+    if (k > 16) return KthLargest<4>(gm, k);
+    const float g[1] = {fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]))};
+    return KthLargest<1>(g, k);
+  }
+  const int lane = threadIdx.x & 63;
+  float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int w = 0; w < TPU / 64; ++w) g[w & 3] = fmaxf(g[w & 3], s.group_max[64 * w + lane]);
+  return KthLargest<4>(g, k);
+}
 
-// What a selection reads, as f(value, column) with all lanes of a wave in step: a unit's registers,
+// What a selection reads, as f(value, column) with all lanes of a wave in step: a unit's registers
+// (`cm`: a lane's maximum of each; what none of the wave's lanes has an element of is passed over),
 template <class T, int NCH, int TPU>
 struct RegSource {
   const U4 (&r)[NCH];
-  int lo, tid;
+  const float (&cm)[NCH];
+  int lo, n, tid;
   template <class F>
-  __device__ void Each(F f) const {
+  __device__ void Each(float floor_v, F f) const {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
+      if (__ballot(cm[c] >= floor_v)) {
+        const int first = lo + FirstCol<T>((c * TPU + tid) * T::kVec, n);
 #pragma unroll
-      for (int j = 0; j < T::kVec; ++j) f(T::Get(r[c], j), lo + (c * TPU + tid) * T::kVec + j);
+        for (int j = 0; j < T::kVec; ++j) f(T::Get(r[c], j), first + j);
+      }
     }
   }
 };
-// the same unit from memory (for the bisection, which is rare: over the registers it would hold
-// every unit's kernel to a copy of its code and theirs),
+// the same unit from memory (for the bisection, which is rare: over the registers it would make
+// every kernel hold its code many times over),
 template <class T, int TPU>
 struct MemSource {
   static constexpr int kLowBit = sizeof(typename T::Store) == 4 ? 0 : 13;  // an f16's or bf16's lower bits are 0
   const typename T::Store *p;
   int lo, n, tid;
   template <class F>
-  __device__ void Each(F f) const {
+  __device__ void Each(float, F f) const {
     for (int base = 0; base < n; base += TPU) {
       const int k = base + tid;
       f(k < n ? T::Load(p + k) : -INFINITY, lo + k);
@@ -308,7 +398,7 @@ struct ListSource {
   const int32_t *i;
   int n, tid;
   template <class F>
-  __device__ void Each(F f) const {
+  __device__ void Each(float, F f) const {
     for (int base = 0; base < n; base += kBlock) {
       const int k = base + tid;
       f(k < n ? v[k] : -INFINITY, k < n ? i[k] : 0);
@@ -316,91 +406,124 @@ struct ListSource {
   }
 };
 
-// Collects the elements that `pred` holds for; their number (all of them, kept or not).
+// Collects a wave's elements that `pred` holds for (none below floor_v); their number, kept or not,
+// in s.count[wave].
 template <int TPU, class SRC, class PRED>
-__device__ inline int Collect(const SRC &src, Scratch &s, PRED pred) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  int base = 0;
-  if (TPU > 64) {
-    if (threadIdx.x == 0) s.count = 0;
-    __syncthreads();
-  }
-  src.Each([&](float v, int i) {
+__device__ inline void Collect(const SRC &src, Scratch<TPU> &s, float floor_v, PRED pred) {
+  const int lane = threadIdx.x & 63, w = TPU == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int n = 0;
+  src.Each(floor_v, [&](float v, int i) {
     const bool mine = pred(v, i);
     const uint64_t m = __ballot(mine);
     if (m) {
-      int at = base;
-      if (TPU > 64) {
-        int got = 0;
-        if (lane == 0) got = atomicAdd(&s.count, Popc(m));
-        at = __builtin_amdgcn_readfirstlane(got);
-      }
-      const int pos = at + Popc(m & below);
-      if (mine && pos < kCap) {
-        s.cand_v[pos] = v;
-        s.cand_i[pos] = i;
-      }
-      base += Popc(m);
+      const int pos = n + Popc(m & ((uint64_t(1) << lane) - 1));
+      if (mine && pos < Scratch<TPU>::kList) s.cand[w][pos] = Cand{v, i};
+      n += Popc(m);
     }
   });
-  UnitSync<TPU>();
-  if (TPU > 64) {
-    base = s.count;
-    __syncthreads();
-  }
-  return base;
+  if (lane == 0) s.count[w] = n;
 }
 
 // The k-th element itself (value and column), among those that reach `floor_v`; at least k do.
 template <int TPU, class SRC>
-__device__ __noinline__ void KthElement(const SRC src, Scratch &s, float floor_v, int k, float *kv, int *ki) {
+__device__ __noinline__ void KthElement(const SRC src, int *red, float floor_v, int k, float *kv, int *ki) {
   uint32_t t = 0;
   for (int bit = 31; bit >= SRC::kLowBit; --bit) {
     const uint32_t c = t | (1u << bit);
     int n = 0;
-    src.Each([&](float v, int) { n += Popc(__ballot(v >= floor_v && OrderKey(v) >= c)); });
-    if (UnitCount<TPU>(n, s.ired) >= k) t = c;
+    src.Each(floor_v, [&](float v, int) { n += Popc(__ballot(v >= floor_v && OrderKey(v) >= c)); });
+    if (UnitCount<TPU>(n, red) >= k) t = c;
   }
+  if (!(t & 0x80000000u)) t |= (1u << SRC::kLowBit) - 1;  // (a negative value's bits are inverted in its key)
   const float val = KeyValue(t);
   int above = 0;
-  src.Each([&](float v, int) { above += Popc(__ballot(v > val)); });
-  const int need = k - UnitCount<TPU>(above, s.ired);  // of the equals, the first `need` columns
+  src.Each(floor_v, [&](float v, int) { above += Popc(__ballot(v > val)); });
+  const int need = k - UnitCount<TPU>(above, red);  // of the equals, the first `need` columns
   int col = 0;  // (the largest column that fewer than `need` equals are in front of; columns < 2^24)
   for (int bit = 23; bit >= 0; --bit) {
     const int c = col | (1 << bit);
     int n = 0;
-    src.Each([&](float v, int i) { n += Popc(__ballot(v == val && i < c)); });
-    if (UnitCount<TPU>(n, s.ired) < need) col = c;
+    src.Each(floor_v, [&](float v, int i) { n += Popc(__ballot(v == val && i < c)); });
+    if (UnitCount<TPU>(n, red) < need) col = c;
   }
   *kv = val;
   *ki = col;
 }
 
+__device__ inline int Ahead(const Cand &a, const Cand &b) {  // 1: a comes before b
+  return (a.v > b.v || (a.v == b.v && a.i < b.i)) ? 1 : 0;
+}
+
 // Puts the unit's K largest elements in order and hands (place, value, column) to `out`, once per
 // place from some lane; places without an element get (-inf, -1).  `threshold`: at least k of the
-// unit's elements reach it, or it is -inf.
+// unit's elements reach it, or it is -inf or NaN.
 template <int TPU, class SRC, class MEM, class OUT>
-__device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch &s, float threshold, int k, OUT out) {
-  const int tid = TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
+__device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s, float threshold, int k, OUT out) {
+  constexpr int kW = TPU / 64, kList = Scratch<TPU>::kList;
+  const int tid = UnitLane<TPU>();
   const float floor_v = fmaxf(threshold, kLowest);  // (-inf is no alternative)
-  int n = Collect<TPU>(src, s, [=](float v, int) { return v >= floor_v; });
-  if (n > kCap) {
+  Collect<TPU>(src, s, floor_v, [=](float v, int) { return v >= floor_v; });
+  if (TPU > 64)
+    for (int a = tid; a < kMaxRanked; a += TPU) s.place[a] = 0;
+  UnitSync<TPU>();
+  int n = 0;
+  bool over = false;
+#pragma unroll
+  for (int w = 0; w < kW; ++w) {
+    n += s.count[w];
+    over |= s.count[w] > kList;
+  }
+  if (over || n > kMaxRanked) {
     float kv;
     int ki;
-    KthElement<TPU>(mem, s, floor_v, k, &kv, &ki);
-    n = Collect<TPU>(mem, s, [=](float v, int i) { return v > kv || (v == kv && i <= ki); });
-    n = min(n, kCap);
+    UnitSync<TPU>();
+    KthElement<TPU>(mem, s.count, floor_v, k, &kv, &ki);
+    UnitSync<TPU>();
+    Collect<TPU>(mem, s, floor_v, [=](float v, int i) { return v > kv || (v == kv && i <= ki); });
+    UnitSync<TPU>();
+    n = k;
   }
-  for (int a = tid; a < n; a += TPU) {
-    const float v = s.cand_v[a];
-    const int i = s.cand_i[a];
-    int place = 0;
-    for (int b = 0; b < n; ++b) {
-      const float w = s.cand_v[b];
-      place += (w > v || (w == v && s.cand_i[b] < i)) ? 1 : 0;
+  if (TPU == 64) {
+    for (int a = tid; a < n; a += 64) {
+      const Cand mine = s.cand[0][a];
+      int place = 0;
+#pragma unroll 4
+      for (int b = 0; b < n; ++b) place += Ahead(s.cand[0][b], mine);
+      if (place < k) out(place, mine.v, mine.i);
     }
-    if (place < k) out(place, v, i);
+  } else {
+    // each wave counts, for every candidate, those of its own list that are ahead
+    const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int own_n = s.count[own];
+    for (int a0 = 0; a0 < n; a0 += 64) {
+      const int a = a0 + lane;
+      int w = 0, i = a;
+#pragma unroll
+      for (int x = 0; x < kW - 1; ++x) {
+        const bool further = w == x && i >= s.count[x];
+        i = further ? i - s.count[x] : i;
+        w = further ? x + 1 : w;
+      }
+      if (a < n) {
+        const Cand mine = s.cand[w][i];
+        int place = 0;
+#pragma unroll 4
+        for (int b = 0; b < own_n; ++b) place += Ahead(s.cand[own][b], mine);
+        if (place) atomicAdd(&s.place[a], place);
+      }
+    }
+    __syncthreads();
+    for (int a = tid; a < n; a += TPU) {
+      if (s.place[a] >= k) continue;
+      int w = 0, i = a;
+#pragma unroll
+      for (int x = 0; x < kW - 1; ++x) {
+        const bool further = w == x && i >= s.count[x];
+        i = further ? i - s.count[x] : i;
+        w = further ? x + 1 : w;
+      }
+      out(s.place[a], s.cand[w][i].v, s.cand[w][i].i);
+    }
   }
   for (int a = n + tid; a < k; a += TPU) out(a, -INFINITY, -1);
 }
@@ -416,7 +539,7 @@ struct ScoresArgs {
   const void *tokens;  // int32 or int64 [rows], or null
   int32_t token64;
   int32_t k;           // alternatives
-  float k2;            // log2(e) / temperature: e_j = exp2((x_j - m) * k2)
+  float k2;            // log2(e) / temperature
   float *logp, *entropy, *stats, *top_v;
   int32_t *top_i;
   Partial *part;       // split rows: [rows][nseg], and [rows][nseg][k] alternatives
@@ -424,8 +547,8 @@ struct ScoresArgs {
   int32_t *part_i;
 };
 
-__device__ inline int64_t Token(const ScoresArgs &a, uint32_t row) {
-  return a.token64 ? static_cast<const int64_t *>(a.tokens)[row] : static_cast<const int32_t *>(a.tokens)[row];
+__device__ inline int64_t IdAt(const void *ids, int32_t id64, size_t at) {
+  return id64 ? static_cast<const int64_t *>(ids)[at] : static_cast<const int32_t *>(ids)[at];
 }
 
 // A row's statistics are its maximum m and s = sum e_j.  (Not log s: 1 / s is what the gradient
@@ -433,18 +556,17 @@ __device__ inline int64_t Token(const ScoresArgs &a, uint32_t row) {
 // m = -inf and s = 0; what is taken relative to its maximum is then taken relative to Base(m) = 0.
 __device__ inline float Base(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ inline float LogSum(float s0) { return s0 == 0.0f ? 0.0f : logf(s0); }
-// H = ls - sum e (x - m) / s: both terms are at least 0, nothing cancels.
-__device__ inline float Entropy(float s0, float s1) { return s0 == 0.0f ? 0.0f : logf(s0) - s1 / s0; }
 
+// s1 = sum e_j log2(e_j): H = log s - ln 2 s1 / s, two terms that are at least 0: nothing cancels.
 template <class T>
 __device__ inline void WriteRowScores(const ScoresArgs &a, const Unit &u, const typename T::Store *x, float m,
                                       float s0, float s1) {
   const float ls = LogSum(s0);
   if (a.tokens) {
-    const int64_t tok = Token(a, u.row);
+    const int64_t tok = IdAt(a.tokens, a.token64, u.row);
     a.logp[u.row] = tok >= 0 && tok < a.r.vocab ? (T::Load(x + tok) - Base(m)) - ls : 0.0f;
   }
-  a.entropy[u.row] = Entropy(s0, s1);
+  a.entropy[u.row] = s0 == 0.0f ? 0.0f : ls - kLn2 * (s1 / s0);
   a.stats[2 * static_cast<size_t>(u.row)] = m;
   a.stats[2 * static_cast<size_t>(u.row) + 1] = s0;
 }
@@ -476,14 +598,13 @@ struct TopWriter {
 };
 
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
-__global__ __launch_bounds__(kBlock) void ScoresKernel(const ScoresArgs a) {
-  constexpr int kUnits = kBlock / TPU;
-  __shared__ Scratch scratch[TOP || TPU > 64 ? kUnits : 1];
-  const int tid = TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  const int which = TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const uint32_t unit = blockIdx.x * kUnits + which;
-  if (TPU == 64 && unit >= a.r.rows * static_cast<uint32_t>(a.r.nseg)) return;
-  Scratch &s = scratch[TOP || TPU > 64 ? which : 0];
+__global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a) {
+  constexpr int kUnits = kThreads<TPU> / TPU;
+  __shared__ Scratch<TPU> scratch[TOP || TPU > 64 ? kUnits : 1];
+  const int tid = UnitLane<TPU>();
+  const uint32_t unit = UnitNumber<TPU>();
+  if (TPU == 64 && unit >= a.r.rows) return;
+  Scratch<TPU> &s = scratch[TOP || TPU > 64 ? UnitInBlock<TPU>() : 0];
   const Unit u = GetUnit(a.r, unit);
   if (u.skip) {
     if (!SPLIT) WriteRowNothing<TPU>(a, u.row, tid);
@@ -493,31 +614,53 @@ __global__ __launch_bounds__(kBlock) void ScoresKernel(const ScoresArgs a) {
   U4 r[NCH];
   LoadUnit<T, NCH, TPU>(x + u.lo, u.n, tid, r);
 
-  // the maxima of four groups of a lane's elements, and of all of them
-  float gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  // the maxima of a lane's 16 bytes, of four groups of its elements, and of all of them
+  float cm[NCH], gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+  for (int c = 0; c < NCH; ++c) {
+    float half[2] = {T::Get(r[c], 0), T::Get(r[c], 1)};
 #pragma unroll
-    for (int j = 0; j < T::kVec; ++j) gm[j & 3] = fmaxf(gm[j & 3], T::Get(r[c], j));
+    for (int j = 2; j < T::kVec; ++j) half[j & 1] = fmaxf(half[j & 1], T::Get(r[c], j));
+    cm[c] = fmaxf(half[0], half[1]);
+    if (NCH >= 4) {
+      gm[c & 3] = fmaxf(gm[c & 3], cm[c]);
+    } else {
+      gm[(2 * c) & 3] = fmaxf(gm[(2 * c) & 3], half[0]);
+      gm[(2 * c + 1) & 3] = fmaxf(gm[(2 * c + 1) & 3], half[1]);
+    }
+  }
   const float lane_max = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
   if (TOP && TPU > 64) s.group_max[tid] = lane_max;
-  const float m = UnitMax<TPU>(lane_max, s.red);
+  const float m = UnitMax<TPU>(lane_max, s.red[0]);
   const float base = Base(m);
 
+  NewPass(r);
+  const Exponent exponent(base, a.k2);
   float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) {
-      const float d = T::Get(r[c], j) - base;
-      const float e = __builtin_amdgcn_exp2f(d * a.k2);
+      const float t = exponent(T::Get(r[c], j)), e = __builtin_amdgcn_exp2f(t);
       s0 += e;
-      // (d is -inf for a masked column: 0 * -inf would be NaN)
-      if (ENT) s1 = fmaf(e, fmaxf(d, kLowest), s1);
+      // (t is -inf for a masked column: 0 * -inf would be NaN)
+      if (ENT) s1 = fmaf(e, fmaxf(t, kLowest), s1);
     }
   }
-  s0 = UnitSum<TPU>(s0, s.red);
-  if (ENT) s1 = UnitSum<TPU>(s1, s.red);
+  s0 = WaveSum(s0);
+  if (ENT) s1 = WaveSum(s1);
+  if (TPU > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      s.red[1][threadIdx.x >> 6] = s0;
+      if (ENT) s.red[2][threadIdx.x >> 6] = s1;
+    }
+    __syncthreads();
+    s0 = SumOf<TPU>(s.red[1]);
+    if (ENT) s1 = SumOf<TPU>(s.red[2]);
+  }
+  const float less = __builtin_amdgcn_exp2f(-exponent.delta);
+  if (ENT) s1 = fmaf(-exponent.delta, s0, s1) * less;
+  s0 *= less;
 
   if (SPLIT) {
     if (tid == 0) a.part[unit] = Partial{m, s0, s1, 0.0f};
@@ -525,18 +668,9 @@ __global__ __launch_bounds__(kBlock) void ScoresKernel(const ScoresArgs a) {
     WriteRowScores<T>(a, u, x, m, s0, s1);
   }
   if (TOP) {
-    float threshold;
-    if (TPU > 64) {
-      const float g[4] = {s.group_max[tid & 63], s.group_max[64 + (tid & 63)], s.group_max[128 + (tid & 63)],
-                          s.group_max[192 + (tid & 63)]};
-      threshold = KthLargest<4>(g, a.k);
-    } else if (a.k > 16) {
-      threshold = KthLargest<4>(gm, a.k);
-    } else {
-      const float g[1] = {lane_max};
-      threshold = KthLargest<1>(g, a.k);
-    }
-    const RegSource<T, NCH, TPU> src{r, u.lo, tid};
+    NewPass(r);
+    const float threshold = GroupThreshold<TPU>(gm, s, a.k);
+    const RegSource<T, NCH, TPU> src{r, cm, u.lo, u.n, tid};
     const MemSource<T, TPU> mem{x + u.lo, u.lo, u.n, tid};
     const size_t at = (SPLIT ? static_cast<size_t>(unit) : static_cast<size_t>(u.row)) * a.k;
     if (SPLIT) {
@@ -553,52 +687,59 @@ __global__ __launch_bounds__(kBlock) void ScoresKernel(const ScoresArgs a) {
   }
 }
 
-// A row's statistics from its segments' (the whole workgroup; `red` is free again on return).
-__device__ inline void JoinPartials(const Partial *part, int nseg, float k2, float *red, float *m_out, float *s0_out,
-                                    float *s1_out) {
+// A row's statistics from its segments' (the whole workgroup).
+__device__ inline void JoinPartials(const Partial *part, int nseg, float k2, float (*red)[kWaves], float *m_out,
+                                    float *s0_out, float *s1_out) {
   float m = -INFINITY;
   for (int i = threadIdx.x; i < nseg; i += kBlock) m = fmaxf(m, part[i].m);
-  m = UnitMax<kBlock>(m, red);
+  m = UnitMax<kBlock>(m, red[0]);
   const float base = Base(m);
   float s0 = 0.0f, s1 = 0.0f;
   for (int i = threadIdx.x; i < nseg; i += kBlock) {
     const Partial p = part[i];
-    const float d = Base(p.m) - base, f = __builtin_amdgcn_exp2f(d * k2);
+    const float t = (Base(p.m) - base) * k2, f = __builtin_amdgcn_exp2f(t);
     // (a segment that adds nothing may have any maximum: its products are not formed)
     if (f != 0.0f && p.s0 != 0.0f) {
       s0 = fmaf(f, p.s0, s0);
-      s1 += f * fmaf(d, p.s0, p.s1);
+      s1 += f * fmaf(t, p.s0, p.s1);
     }
   }
+  s0 = WaveSum(s0);
+  s1 = WaveSum(s1);
+  if ((threadIdx.x & 63) == 0) {
+    red[1][threadIdx.x >> 6] = s0;
+    red[2][threadIdx.x >> 6] = s1;
+  }
+  __syncthreads();
   *m_out = m;
-  *s0_out = UnitSum<kBlock>(s0, red);
-  *s1_out = UnitSum<kBlock>(s1, red);
+  *s0_out = SumOf<kBlock>(red[1]);
+  *s1_out = SumOf<kBlock>(red[2]);
 }
 
 template <class T, bool TOP>
 __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
-  __shared__ Scratch s;
+  __shared__ Scratch<kBlock> s;
   const int tid = threadIdx.x;
-  Unit u = GetUnit(a.r, blockIdx.x * static_cast<uint32_t>(a.r.nseg));
+  const Unit u = GetUnit(a.r, blockIdx.x * static_cast<uint32_t>(a.r.nseg));
   if (u.skip) {
     WriteRowNothing<kBlock>(a, u.row, tid);
     return;
   }
   const int nseg = a.r.nseg;
+  const size_t n = static_cast<size_t>(nseg) * a.k;
+  const ListSource src{a.part_v + u.row * n, a.part_i + u.row * n, static_cast<int>(n), tid};
+  if (TOP) {
+    float mine = -INFINITY;
+    src.Each(0.0f, [&](float v, int) { mine = fmaxf(mine, v); });
+    s.group_max[tid] = mine;
+  }
   float m, s0, s1;
   JoinPartials(a.part + static_cast<size_t>(u.row) * nseg, nseg, a.k2, s.red, &m, &s0, &s1);
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
   if (tid == 0) WriteRowScores<T>(a, u, x, m, s0, s1);
   if (TOP) {
-    const size_t n = static_cast<size_t>(nseg) * a.k;
-    const ListSource src{a.part_v + u.row * n, a.part_i + u.row * n, static_cast<int>(n), tid};
-    float mine = -INFINITY;
-    src.Each([&](float v, int) { mine = fmaxf(mine, v); });
-    s.group_max[tid] = mine;
-    __syncthreads();
-    const float g[4] = {s.group_max[tid & 63], s.group_max[64 + (tid & 63)], s.group_max[128 + (tid & 63)],
-                        s.group_max[192 + (tid & 63)]};
-    const float threshold = KthLargest<4>(g, a.k);
+    const float none[4] = {};
+    const float threshold = GroupThreshold<kBlock>(none, s, a.k);
     const float ls = LogSum(s0);
     SelectTop<kBlock>(src, src, s, threshold, a.k,
                       TopWriter{a.top_v + static_cast<size_t>(u.row) * a.k, a.top_i + static_cast<size_t>(u.row) * a.k,
@@ -613,22 +754,22 @@ struct GradOut {
   int64_t batch_stride, row_stride;
 };
 
-// Writes f(value, column) for a unit's elements; a lane's columns as in LoadUnit.
+// Writes g[0 .. kVec) = f(r[c], first column in the unit) for a unit's elements.
 template <class T, int NCH, int TPU, class F>
 __device__ inline void StoreUnit(typename T::Store *p, int n, int tid, const U4 (&r)[NCH], F f) {
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int e = (c * TPU + tid) * T::kVec;
     if (e < n) {
+      const int first = FirstCol<T>(e, n);
       float g[T::kVec];
-#pragma unroll
-      for (int j = 0; j < T::kVec; ++j) g[j] = f(T::Get(r[c], j), e + j);
+      f(r[c], first, g);
       if (e + T::kVec <= n) {
         *reinterpret_cast<typename T::Vec *>(p + e) = T::Pack(g);
-      } else {
+      } else {  // (the columns in front are another lane's)
 #pragma unroll
         for (int j = 0; j < T::kVec; ++j)
-          if (e + j < n) p[e + j] = T::Round(g[j]);
+          if (first + j >= e && first + j < n) p[first + j] = T::Round(g[j]);
       }
     }
   }
@@ -656,15 +797,14 @@ struct ScoresGradArgs {
   const float *g_logp, *g_entropy; // upstream, [rows] each, or null (0)
 };
 
-// dx_j = g_logp ([j = token] - p_j) - g_H p_j (log p_j + H) = p_j (A - g_H log p_j) + g_logp [j = token]
-// with A = -g_logp - g_H H.
+// dx_j = g_logp ([j = token] - p_j) - g_H p_j (log p_j + H).  With p_j = e_j / s, log p_j = ln 2 t_j -
+// log s (t_j the exponent) that is e_j (A + B t_j) + g_logp [j = token]: A = (-g_logp - g_H (H - log s)) / s,
+// B = -ln 2 g_H / s.
 template <class T, int NCH, int TPU>
-__global__ __launch_bounds__(kBlock) void ScoresGradKernel(const ScoresGradArgs a) {
-  constexpr int kUnits = kBlock / TPU;
-  const int tid = TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  const int which = TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const uint32_t unit = blockIdx.x * kUnits + which;
-  if (unit >= a.r.rows * static_cast<uint32_t>(a.r.nseg)) return;
+__global__ __launch_bounds__(kThreads<TPU>) void ScoresGradKernel(const ScoresGradArgs a) {
+  const int tid = UnitLane<TPU>();
+  const uint32_t unit = UnitNumber<TPU>();
+  if (TPU == 64 && unit >= a.r.rows) return;
   const Unit u = GetUnit(a.r, unit);
   typename T::Store *dx =
       const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)) + u.lo;
@@ -676,21 +816,26 @@ __global__ __launch_bounds__(kBlock) void ScoresGradKernel(const ScoresGradArgs 
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u) + u.lo;
   U4 r[NCH];
   LoadUnit<T, NCH, TPU>(x, u.n, tid, r);
-  int64_t tok = a.tokens ? (a.token64 ? static_cast<const int64_t *>(a.tokens)[u.row]
-                                      : static_cast<const int32_t *>(a.tokens)[u.row])
-                         : -1;
+  int64_t tok = a.tokens ? IdAt(a.tokens, a.token64, u.row) : -1;
   if (tok < 0 || tok >= a.r.vocab) tok = -1;
   const float gl = a.g_logp && tok >= 0 ? a.g_logp[u.row] : 0.0f;
   const float gh = a.g_entropy ? a.g_entropy[u.row] : 0.0f;
-  const float A = a.g_entropy ? -gl - gh * a.entropy[u.row] : -gl;
-  const int at = tok < 0 ? -1 : static_cast<int>(tok) - u.lo;  // (outside the unit: matches no column)
-  const float inv = 1.0f / s0, ls = logf(s0);
-  StoreUnit<T, NCH, TPU>(dx, u.n, tid, r, [=](float v, int e) {
-    const float d = v - m;
-    const float p = __builtin_amdgcn_exp2f(d * kLog2e) * inv;
-    const float lp = fmaxf(d - ls, -128.0f);  // (below -104 p is 0, and 0 times -inf would be NaN)
-    const float g = p * fmaf(-gh, lp, A);
-    return e == at ? g + gl : g;
+  const int at = tok < 0 ? -T::kVec : static_cast<int>(tok) - u.lo;  // (may be outside the unit)
+  const Exponent exponent(m, kLog2e);
+  const float inv = __builtin_amdgcn_exp2f(-exponent.delta) / s0, ls = logf(s0);
+  const float B = -kLn2 * gh * inv;
+  const float A = (a.g_entropy ? -gl - gh * (a.entropy[u.row] - ls) : -gl) * inv - B * exponent.delta;
+  StoreUnit<T, NCH, TPU>(dx, u.n, tid, r, [=](const U4 &v, int first, float *g) {
+#pragma unroll
+    for (int j = 0; j < T::kVec; ++j) {
+      const float t = exponent(T::Get(v, j));
+      // (below -150 e is 0, and 0 times -inf would be NaN)
+      g[j] = __builtin_amdgcn_exp2f(t) * fmaf(B, fmaxf(t, -256.0f), A);
+    }
+    if (static_cast<uint32_t>(at - first) < static_cast<uint32_t>(T::kVec)) {
+#pragma unroll
+      for (int j = 0; j < T::kVec; ++j) g[j] += first + j == at ? gl : 0.0f;
+    }
   });
 }
 
@@ -717,13 +862,15 @@ __device__ inline float TeacherValue(const DistillArgs &a, size_t at) {
 }
 
 // A unit's teacher: lane `tid` holds slots tid, tid + TPU, ...; all of them also in LDS.
+template <int TPU>
 struct TeacherList {
   int id[kMaxSlots];
   float q[kMaxSlots];
+  float red[5][TPU / 64];
 };
 template <int TPU>
 struct Slots {
-  static constexpr int kN = kMaxSlots / TPU;
+  static constexpr int kN = TPU < kMaxSlots ? kMaxSlots / TPU : 1;
   int id[kN];   // -1: empty
   float u[kN];  // (logit - largest) / temperature
   float q[kN];
@@ -740,8 +887,7 @@ __device__ inline void LoadSlots(const DistillArgs &a, uint32_t row, int tid, Sl
     const int k = i * TPU + tid;
     if (k < a.slots) {
       const size_t at = static_cast<size_t>(row) * a.slots + k;
-      const int64_t id =
-          a.id64 ? static_cast<const int64_t *>(a.ids)[at] : static_cast<const int32_t *>(a.ids)[at];
+      const int64_t id = IdAt(a.ids, a.id64, at);
       if (id >= 0 && id < a.r.vocab) {
         t.id[i] = static_cast<int>(id);
         t.u[i] = TeacherValue(a, at);
@@ -751,7 +897,7 @@ __device__ inline void LoadSlots(const DistillArgs &a, uint32_t row, int tid, Sl
 }
 // q = softmax(u / temperature) over the filled slots.
 template <int TPU>
-__device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, TeacherList &list, float *red, int tid) {
+__device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, TeacherList<TPU> &list, int tid) {
   float um = -INFINITY, sum = 0.0f;
   bool nan = false;
 #pragma unroll
@@ -759,7 +905,7 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, Teacher
     um = fmaxf(um, t.u[i]);
     nan |= isnan(t.u[i]);
   }
-  um = UnitMax<TPU>(nan ? INFINITY : um, red);  // (inf - inf below: NaN for the whole row)
+  um = UnitMax<TPU>(nan ? INFINITY : um, list.red[0]);  // (inf - inf below: NaN for the whole row)
   t.any = um != -INFINITY;
 #pragma unroll
   for (int i = 0; i < Slots<TPU>::kN; ++i) {
@@ -767,7 +913,7 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, Teacher
     t.q[i] = um == INFINITY && t.id[i] >= 0 ? NAN : expf(t.u[i]);
     sum += t.q[i];
   }
-  sum = UnitSum<TPU>(sum, red);
+  sum = UnitSum<TPU>(sum, list.red[1]);
   t.log_usum = logf(sum);
 #pragma unroll
   for (int i = 0; i < Slots<TPU>::kN; ++i) {
@@ -800,14 +946,17 @@ __device__ inline float Divergence(const DistillArgs &a, const Slots<TPU> &t, co
 // the same value).
 template <class T, int NCH, int TPU>
 __device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, const U4 (&r)[NCH], const Slots<TPU> &t,
-                                        const float (&xs)[Slots<TPU>::kN], const TeacherList &list, float m, float s0,
-                                        float coef, int tid) {
+                                        const float (&xs)[Slots<TPU>::kN], const TeacherList<TPU> &list, float m,
+                                        float s0, float coef, int tid) {
   typename T::Store *dx =
       const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)) + u.lo;
+  const Exponent exponent(Base(m), a.k2);
   // (a student without a finite logit gives nothing any probability)
-  const float base = Base(m), k2 = a.k2, inv = s0 == 0.0f ? 0.0f : 1.0f / s0, scale = coef * inv;
-  StoreUnit<T, NCH, TPU>(dx, u.n, tid, r,
-                         [=](float v, int) { return scale * __builtin_amdgcn_exp2f((v - base) * k2); });
+  const float inv = s0 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-exponent.delta) / s0, scale = coef * inv;
+  StoreUnit<T, NCH, TPU>(dx, u.n, tid, r, [=](const U4 &v, int, float *g) {
+#pragma unroll
+    for (int j = 0; j < T::kVec; ++j) g[j] = scale * __builtin_amdgcn_exp2f(exponent(T::Get(v, j)));
+  });
   UnitSync<TPU>();
 #pragma unroll
   for (int i = 0; i < Slots<TPU>::kN; ++i) {
@@ -817,29 +966,38 @@ __device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, con
     if (__ballot(mine)) {
       float q = 0.0f;
       for (int k = 0; k < a.slots; ++k) q += list.id[k] == t.id[i] ? list.q[k] : 0.0f;
-      if (mine) dx[at] = T::Round(coef * (__builtin_amdgcn_exp2f((xs[i] - base) * k2) * inv - q));
+      if (mine) dx[at] = T::Round(coef * (__builtin_amdgcn_exp2f(exponent(xs[i])) * inv - q));
     }
   }
 }
 
+// The students' logits at a lane's slots.
+template <class T, int TPU>
+__device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU> &t, float (&xs)[Slots<TPU>::kN]) {
+#pragma unroll
+  for (int i = 0; i < Slots<TPU>::kN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
+}
+
 // Whole rows: loss, and with GRAD the gradient from the registers that the statistics were taken of.
 template <class T, int NCH, int TPU, bool GRAD>
-__global__ __launch_bounds__(kBlock) void DistillKernel(const DistillArgs a) {
-  constexpr int kUnits = kBlock / TPU;
-  __shared__ TeacherList lists[kUnits];
-  __shared__ float red[kWaves];
-  const int tid = TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  const int which = TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const uint32_t unit = blockIdx.x * kUnits + which;
-  if (unit >= a.r.rows) return;
+__global__ __launch_bounds__(kThreads<TPU>) void DistillKernel(const DistillArgs a) {
+  __shared__ TeacherList<TPU> lists[kThreads<TPU> / TPU];
+  const int tid = UnitLane<TPU>();
+  const uint32_t unit = UnitNumber<TPU>();
+  if (TPU == 64 && unit >= a.r.rows) return;
   const Unit u = GetUnit(a.r, unit);
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
-  TeacherList &list = lists[which];
+  TeacherList<TPU> &list = lists[UnitInBlock<TPU>()];
   Slots<TPU> t;
   t.any = false;
+  const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
+  U4 r[NCH];
+  float xs[Slots<TPU>::kN];
   if (w != 0.0f) {
     LoadSlots<TPU>(a, u.row, tid, t);
-    SoftmaxSlots<TPU>(a, t, list, red, tid);
+    LoadUnit<T, NCH, TPU>(x, u.n, tid, r);
+    LoadAtSlots<T, TPU>(x, t, xs);
+    SoftmaxSlots<TPU>(a, t, list, tid);
   }
   if (!t.any) {  // (the same in all lanes of the unit)
     if (tid == 0) {
@@ -851,27 +1009,22 @@ __global__ __launch_bounds__(kBlock) void DistillKernel(const DistillArgs a) {
           const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)), u.n, tid);
     return;
   }
-  const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
-  U4 r[NCH];
-  LoadUnit<T, NCH, TPU>(x, u.n, tid, r);
-  float xs[Slots<TPU>::kN];
-#pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
   float m = -INFINITY;
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) m = fmaxf(m, T::Get(r[c], j));
-  m = UnitMax<TPU>(m, red);
-  const float base = Base(m);
+  m = UnitMax<TPU>(m, list.red[2]);
+  NewPass(r);
+  const Exponent exponent(Base(m), a.k2);
   float s0 = 0.0f;
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
-    for (int j = 0; j < T::kVec; ++j) s0 += __builtin_amdgcn_exp2f((T::Get(r[c], j) - base) * a.k2);
-  s0 = UnitSum<TPU>(s0, red);
+    for (int j = 0; j < T::kVec; ++j) s0 += __builtin_amdgcn_exp2f(exponent(T::Get(r[c], j)));
+  s0 = UnitSum<TPU>(s0, list.red[3]) * __builtin_amdgcn_exp2f(-exponent.delta);
   const float ls = LogSum(s0);
-  const float loss = Divergence<TPU>(a, t, xs, m, ls, red);
+  const float loss = Divergence<TPU>(a, t, xs, m, ls, list.red[4]);
   if (tid == 0) {
     if (a.loss) a.loss[u.row] = w * loss;
     if (a.stats) {
@@ -880,6 +1033,7 @@ __global__ __launch_bounds__(kBlock) void DistillKernel(const DistillArgs a) {
     }
   }
   if (GRAD) {
+    NewPass(r);
     const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
     WriteDistillGrad<T, NCH, TPU>(a, u, r, t, xs, list, m, s0, coef, tid);
   }
@@ -888,8 +1042,8 @@ __global__ __launch_bounds__(kBlock) void DistillKernel(const DistillArgs a) {
 // Split rows: the statistics of a row from its segments', and its loss.
 template <class T>
 __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a) {
-  __shared__ TeacherList list;
-  __shared__ float red[kWaves];
+  __shared__ TeacherList<kBlock> list;
+  __shared__ float red[3][kWaves];
   const int tid = threadIdx.x;
   const Unit u = GetUnit(a.r, blockIdx.x * static_cast<uint32_t>(a.r.nseg));
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
@@ -897,16 +1051,14 @@ __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a)
   t.any = false;
   if (w != 0.0f) {
     LoadSlots<kBlock>(a, u.row, tid, t);
-    SoftmaxSlots<kBlock>(a, t, list, red, tid);
+    SoftmaxSlots<kBlock>(a, t, list, tid);
   }
   float m = 0.0f, s0 = 0.0f, loss = 0.0f;
   if (t.any) {
-    float s1;
+    float s1, xs[1];
+    LoadAtSlots<T, kBlock>(RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u), t, xs);
     JoinPartials(a.part + static_cast<size_t>(u.row) * a.r.nseg, a.r.nseg, a.k2, red, &m, &s0, &s1);
-    const float ls = LogSum(s0);
-    const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
-    const float xs[1] = {t.id[0] >= 0 ? T::Load(x + t.id[0]) : 0.0f};
-    loss = Divergence<kBlock>(a, t, xs, m, ls, red);
+    loss = Divergence<kBlock>(a, t, xs, m, LogSum(s0), list.red[4]);
   }
   if (tid == 0) {
     if (a.loss) a.loss[u.row] = t.any ? w * loss : 0.0f;
@@ -917,37 +1069,34 @@ __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a)
 
 // The gradient of rows or segments whose statistics are known.
 template <class T, int NCH, int TPU>
-__global__ __launch_bounds__(kBlock) void DistillGradKernel(const DistillArgs a) {
-  constexpr int kUnits = kBlock / TPU;
-  __shared__ TeacherList lists[kUnits];
-  __shared__ float red[kWaves];
-  const int tid = TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  const int which = TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const uint32_t unit = blockIdx.x * kUnits + which;
-  if (unit >= a.r.rows * static_cast<uint32_t>(a.r.nseg)) return;
+__global__ __launch_bounds__(kThreads<TPU>) void DistillGradKernel(const DistillArgs a) {
+  __shared__ TeacherList<TPU> lists[kThreads<TPU> / TPU];
+  const int tid = UnitLane<TPU>();
+  const uint32_t unit = UnitNumber<TPU>();
+  if (TPU == 64 && unit >= a.r.rows) return;
   const Unit u = GetUnit(a.r, unit);
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
-  TeacherList &list = lists[which];
+  TeacherList<TPU> &list = lists[UnitInBlock<TPU>()];
   Slots<TPU> t;
   t.any = false;
+  const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
+  U4 r[NCH];
+  float xs[Slots<TPU>::kN];
   if (w != 0.0f) {
     LoadSlots<TPU>(a, u.row, tid, t);
-    SoftmaxSlots<TPU>(a, t, list, red, tid);
+    LoadUnit<T, NCH, TPU>(x + u.lo, u.n, tid, r);
+    LoadAtSlots<T, TPU>(x, t, xs);
+    // (its barriers stand between every lane's loads of the slots' logits and the first stores: the
+    // gradient may be written over the logits)
+    SoftmaxSlots<TPU>(a, t, list, tid);
   }
   if (!t.any) {
     StoreZeros<T, NCH, TPU>(
         const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)) + u.lo, u.n, tid);
     return;
   }
-  const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
-  U4 r[NCH];
-  LoadUnit<T, NCH, TPU>(x + u.lo, u.n, tid, r);
-  float xs[Slots<TPU>::kN];
-#pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
   const float m = a.stats[2 * static_cast<size_t>(u.row)], s0 = a.stats[2 * static_cast<size_t>(u.row) + 1];
   const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
-  UnitSync<TPU>();  // (the gradient may be written over the logits: every lane has its slots' first)
   WriteDistillGrad<T, NCH, TPU>(a, u, r, t, xs, list, m, s0, coef, tid);
 }
 
@@ -1233,8 +1382,8 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
       return SetError(KD_E_INVALID, "bad argument: id_bytes must be 4 or 8");
     if (teacher->dtype != KD_DTYPE_F32 && teacher->dtype != KD_DTYPE_F16 && teacher->dtype != KD_DTYPE_BF16)
       return SetError(KD_E_INVALID, "bad argument: dtype of the teacher's logits");
-    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(kLog2e / temperature))
-      return SetError(KD_E_INVALID, "bad argument: temperature must be positive and finite");
+    if (!(temperature >= 1e-6f && temperature <= 1e6f))
+      return SetError(KD_E_INVALID, "bad argument: temperature must be between 1e-6 and 1e6");
     if (!n) return KD_OK;
     if (!teacher->ids || !teacher->logits) return SetError(KD_E_INVALID, "bad argument: the teacher's list is NULL");
     if (!loss && !grad) return SetError(KD_E_INVALID, "bad argument: neither loss nor gradient asked for");

@@ -79,7 +79,7 @@ def token_scores_grad(logits, scores, tokens=None, lengths=None, grad_logp=None,
 
 def distill_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, lengths=None):
     """Per row, weight * KL(q || p) over the tokens a teacher lists: q = softmax(teacher_logits /
-    temperature) over the row's list, p = softmax(logits / temperature) over the vocabulary.
+    temperature) over the row's list, p = softmax(logits / temperature) over the vocabulary, 1e-6 <= temperature <= 1e6.
 
     `teacher_ids` (int32 or int64) and `teacher_logits` (float32, float16, bfloat16; log-probabilities
     serve as well) [..., K], K <= 256; an id outside [0, V), such as -1, marks an empty slot, one that
