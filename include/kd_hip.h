@@ -342,8 +342,9 @@ int kd_batch_set_log_softmax(kd_batch *b, int32_t on);
  * default) and returns: no allocation, no synchronisation, no state of the library's, so calls may
  * be captured into a graph and made from several threads.  The workspace is the caller's, 16-byte
  * aligned, and in use until the call's work on the stream is done: calls that may overlap (another
- * stream, another captured graph) need one each.  Sums and statistics are f32; results do not
- * depend on how rows are dealt out and are the same from run to run.
+ * stream, another captured graph) need one each.  Sums and statistics are f32; a call gives the same
+ * bits from run to run (a row's last bits may depend on the number of rows it is called with: few
+ * long rows are cut into more pieces).
  * vocab <= 2^24; at most 2^24 - 1 rows (x ceil(row bytes / 32 KiB) where a row is longer than that;
  * four times as many rows of up to 8 KiB). */
 #define KD_DTYPE_F32 0
@@ -398,7 +399,7 @@ typedef struct kd_teacher_rows {
  * loss): maximum and sum of the row, written with a loss; with `loss` NULL they are read, and the
  * call computes the gradient alone (the same inputs as the call that wrote them).  `grad` may be
  * the logits themselves, as in kd_token_scores_grad.  Loss and gradient in one call read a row of up to 32 KiB once. */
-size_t kd_distill_loss_workspace(const kd_frame_rows *rows);
+size_t kd_distill_loss_workspace(const kd_frame_rows *rows, int32_t with_grad);
 int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, const float *weights,
                     float temperature, float *loss, float *stats, const float *upstream, void *grad,
                     int64_t grad_batch_stride, int64_t grad_row_stride, void *workspace,

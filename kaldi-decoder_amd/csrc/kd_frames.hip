@@ -144,15 +144,23 @@ template <class T>
 __device__ inline int FirstCol(int e, int n) {
   return min(e, max(n - T::kVec, 0));
 }
+// Whether any lane of a unit of n columns has some in r[c] (passes leave out the others: the same
+// for the whole unit, and one kernel for 8 16-byte loads a lane does the work of fewer as well).
+template <class T, int TPU>
+__device__ inline bool Used(int c, int n) {
+  return c == 0 || c * TPU * T::kVec < n;
+}
 template <class T, int NCH, int TPU>
 __device__ inline void LoadUnit(const typename T::Store *p, int n, int tid, U4 (&r)[NCH]) {
   if (n >= T::kVec) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
-      r[c] = *reinterpret_cast<const typename T::Vec *>(p + FirstCol<T>((c * TPU + tid) * T::kVec, n));
+    for (int c = 0; c < NCH; ++c) {
+      if (Used<T, TPU>(c, n))
+        r[c] = *reinterpret_cast<const typename T::Vec *>(p + FirstCol<T>((c * TPU + tid) * T::kVec, n));
+    }
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      if ((c + 1) * TPU * T::kVec <= n) continue;  // (no lane of this one reaches the end)
+      if ((c + 1) * TPU * T::kVec <= n || !Used<T, TPU>(c, n)) continue;  // (no lane of this one reaches the end)
       const int e = (c * TPU + tid) * T::kVec, others = e - FirstCol<T>(e, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -166,8 +174,7 @@ __device__ inline void LoadUnit(const typename T::Store *p, int n, int tid, U4 (
       }
     }
   } else {  // a row of less than 16 bytes: all lane 0's
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) r[c] = U4{T::kFill, T::kFill, T::kFill, T::kFill};
+    r[0] = U4{T::kFill, T::kFill, T::kFill, T::kFill};
     if (tid == 0) {
 #pragma unroll
       for (int j = 0; j < T::kVec - 1; ++j) {
@@ -191,27 +198,50 @@ __device__ inline void NewPass(U4 (&r)[NCH]) {
 }
 
 // ---- reductions over a unit --------------------------------------------------------------------
-// Wave level: five DPP steps inside rows of 16, then across them (lane 63 has the whole).
-template <int CTRL, int ROW_MASK>
-__device__ inline float Dpp(float identity, float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(identity), __float_as_int(v), CTRL, ROW_MASK, 0xf,
-                                                    false));
+// The larger of two; NaN if either is.  (fmaxf, which drops NaN, costs an instruction more for each
+// operand that might be a signaling one; this is one v_maximum3, for three operands too.)
+__device__ inline float Max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ inline float Min(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+
+template <int CTRL, int ROW_MASK = 0xf, int BANK_MASK = 0xf>
+__device__ inline int DppI(int old, int v) {
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROW_MASK, BANK_MASK, false);
 }
-template <class OP>
-__device__ inline float WaveReduce(float v, float identity, OP op) {
-  v = op(v, Dpp<0x111, 0xf>(identity, v));  // row_shr:1
-  v = op(v, Dpp<0x112, 0xf>(identity, v));
-  v = op(v, Dpp<0x114, 0xf>(identity, v));
-  v = op(v, Dpp<0x118, 0xf>(identity, v));
-  v = op(v, Dpp<0x142, 0xa>(identity, v));  // row_bcast:15
-  v = op(v, Dpp<0x143, 0xc>(identity, v));  // row_bcast:31
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+template <int CTRL, int ROW_MASK = 0xf, int BANK_MASK = 0xf>
+__device__ inline float Dpp(float old, float v) {
+  return __int_as_float(DppI<CTRL, ROW_MASK, BANK_MASK>(__float_as_int(old), __float_as_int(v)));
 }
+// Over 16 lanes (a DPP row), by rotations: every lane has the result.
+constexpr int kRowRor = 0x120;
+__device__ inline float RowMax(float v) {
+  v = Max(v, Dpp<kRowRor + 8>(v, v));
+  v = Max(v, Dpp<kRowRor + 4>(v, v));
+  v = Max(v, Dpp<kRowRor + 2>(v, v));
+  return Max(v, Dpp<kRowRor + 1>(v, v));
+}
+__device__ inline float RowSum(float v) {
+  v += Dpp<kRowRor + 8>(v, v);
+  v += Dpp<kRowRor + 4>(v, v);
+  v += Dpp<kRowRor + 2>(v, v);
+  return v + Dpp<kRowRor + 1>(v, v);
+}
+__device__ inline int RowSum(int v) {
+  v += DppI<kRowRor + 8>(v, v);
+  v += DppI<kRowRor + 4>(v, v);
+  v += DppI<kRowRor + 2>(v, v);
+  return v + DppI<kRowRor + 1>(v, v);
+}
+// Over a wave: rows 1 and 3 take over what row 0 and 2 have, then rows 2 and 3; lane 63 has all.
+__device__ inline float Lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
 __device__ inline float WaveMax(float v) {
-  return WaveReduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+  v = RowMax(v);
+  v = Max(v, Dpp<0x142, 0xa>(v, v));  // row_bcast:15
+  return Lane63(Max(v, Dpp<0x143, 0xc>(v, v)));  // row_bcast:31
 }
 __device__ inline float WaveSum(float v) {
-  return WaveReduce(v, 0.0f, [](float a, float b) { return a + b; });
+  v = RowSum(v);
+  v += Dpp<0x142, 0xa>(0.0f, v);
+  return Lane63(v + Dpp<0x143, 0xc>(0.0f, v));
 }
 
 // A unit of one wave (TPU 64) is never synchronised with the workgroup's others.
@@ -234,7 +264,7 @@ __device__ inline float UnitMax(float v, float *red) {
   __syncthreads();
   v = red[0];
 #pragma unroll
-  for (int w = 1; w < TPU / 64; ++w) v = fmaxf(v, red[w]);
+  for (int w = 1; w < TPU / 64; ++w) v = Max(v, red[w]);
   return v;
 }
 template <int TPU>
@@ -297,19 +327,16 @@ struct Exponent {
 constexpr int kCap = 128;       // candidates a wave's list holds; a unit of one wave: twice that
 constexpr int kMaxRanked = 512; // candidates a unit ranks
 
-struct Cand {
-  float v;
-  int32_t i;
-};
 template <int TPU>
 struct Scratch {
   static constexpr int kW = TPU / 64;
   static constexpr int kList = kW == 1 ? 2 * kCap : kCap;
   float red[3][kW];
   int count[kW];
+  float threshold;
   float group_max[kW == 1 ? 1 : 64 * kW];
   int place[kW == 1 ? 1 : kMaxRanked];
-  Cand cand[kW][kList];
+  uint64_t cand[kW][kList];  // Key
 };
 
 // A whole number that orders as the value does (-0 and +0 alike).
@@ -320,6 +347,14 @@ __device__ inline uint32_t OrderKey(float v) {
 __device__ inline float KeyValue(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
+
+// A candidate as one number that orders as candidates do: larger value first, then lower column.
+// (0: none.)
+__device__ inline uint64_t Key(float v, int col) {
+  return static_cast<uint64_t>(OrderKey(v)) << 32 | static_cast<uint32_t>(~col);
+}
+__device__ inline float ValueOf(uint64_t key) { return KeyValue(static_cast<uint32_t>(key >> 32)); }
+__device__ inline int ColumnOf(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
 
 // A value that at least k (<= 64 * G) of a wave's 64 * G values reach, and few more than k do: the
 // upper half of the k-th largest's key, bit by bit.
@@ -342,19 +377,25 @@ __device__ inline float KthLargest(const float (&v)[G], int k) {
   // (a key below that of -inf is a NaN's; SelectTop takes either for "all")
   return KeyValue(t);
 }
-// The same of a unit's group maxima: a lane's own in a unit of one wave, else those in LDS.
+// The same of a unit's group maxima: a lane's own in a unit of one wave, else those in LDS -- by one
+// wave, while the others' issue slots are free for other units (by each wave: 12.2 instead of 10.6 us
+// where a unit of four waves takes a row of 5003 columns).
 template <int TPU>
-__device__ inline float GroupThreshold(const float (&gm)[4], const Scratch<TPU> &s, int k) {
+__device__ inline float GroupThreshold(const float (&gm)[4], Scratch<TPU> &s, int k) {
   if (TPU == 64) {
     if (k > 16) return KthLargest<4>(gm, k);
-    const float g[1] = {fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]))};
+    const float g[1] = {Max(Max(gm[0], gm[1]), Max(gm[2], gm[3]))};
     return KthLargest<1>(g, k);
   }
-  const int lane = threadIdx.x & 63;
-  float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (threadIdx.x < 64) {
+    float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int w = 0; w < TPU / 64; ++w) g[w & 3] = fmaxf(g[w & 3], s.group_max[64 * w + lane]);
-  return KthLargest<4>(g, k);
+    for (int w = 0; w < TPU / 64; ++w) g[w & 3] = Max(g[w & 3], s.group_max[64 * w + threadIdx.x]);
+    const float t = KthLargest<4>(g, k);
+    if (threadIdx.x == 0) s.threshold = t;
+  }
+  __syncthreads();
+  return s.threshold;
 }
 
 // What a selection reads, as f(value, column) with all lanes of a wave in step: a unit's registers
@@ -391,17 +432,25 @@ struct MemSource {
     }
   }
 };
-// or a list in memory (the alternatives of a row's segments).
+// or the sorted lists of a row's segments, in memory (the first of all, then the second of all, ...:
+// a thread's share, whose maximum is one of the threshold's groups, has few of any one list's head).
 struct ListSource {
   static constexpr int kLowBit = 0;
-  const float *v;
-  const int32_t *i;
-  int n, tid;
+  const uint64_t *list;  // [nseg][k]
+  int nseg, k, tid;
   template <class F>
   __device__ void Each(float, F f) const {
-    for (int base = 0; base < n; base += kBlock) {
-      const int k = base + tid;
-      f(k < n ? v[k] : -INFINITY, k < n ? i[k] : 0);
+    int at = tid / nseg, seg = tid - at * nseg;
+    const int ats = kBlock / nseg, segs = kBlock - ats * nseg;
+    for (int base = 0; base < nseg * k; base += kBlock) {
+      const uint64_t key = at < k ? list[static_cast<size_t>(seg) * k + at] : 0;  // (0: its value is a NaN)
+      f(ValueOf(key), ColumnOf(key));
+      at += ats;
+      seg += segs;
+      if (seg >= nseg) {
+        seg -= nseg;
+        ++at;
+      }
     }
   }
 };
@@ -417,16 +466,16 @@ __device__ inline void Collect(const SRC &src, Scratch<TPU> &s, float floor_v, P
     const uint64_t m = __ballot(mine);
     if (m) {
       const int pos = n + Popc(m & ((uint64_t(1) << lane) - 1));
-      if (mine && pos < Scratch<TPU>::kList) s.cand[w][pos] = Cand{v, i};
+      if (mine && pos < Scratch<TPU>::kList) s.cand[w][pos] = Key(v, i);
       n += Popc(m);
     }
   });
   if (lane == 0) s.count[w] = n;
 }
 
-// The k-th element itself (value and column), among those that reach `floor_v`; at least k do.
+// The key of the k-th element itself, among those that reach `floor_v`; at least k do.
 template <int TPU, class SRC>
-__device__ __noinline__ void KthElement(const SRC src, int *red, float floor_v, int k, float *kv, int *ki) {
+__device__ __noinline__ uint64_t KthElement(const SRC src, int *red, float floor_v, int k) {
   uint32_t t = 0;
   for (int bit = 31; bit >= SRC::kLowBit; --bit) {
     const uint32_t c = t | (1u << bit);
@@ -446,17 +495,12 @@ __device__ __noinline__ void KthElement(const SRC src, int *red, float floor_v, 
     src.Each(floor_v, [&](float v, int i) { n += Popc(__ballot(v == val && i < c)); });
     if (UnitCount<TPU>(n, red) < need) col = c;
   }
-  *kv = val;
-  *ki = col;
+  return Key(val, col);
 }
 
-__device__ inline int Ahead(const Cand &a, const Cand &b) {  // 1: a comes before b
-  return (a.v > b.v || (a.v == b.v && a.i < b.i)) ? 1 : 0;
-}
-
-// Puts the unit's K largest elements in order and hands (place, value, column) to `out`, once per
-// place from some lane; places without an element get (-inf, -1).  `threshold`: at least k of the
-// unit's elements reach it, or it is -inf or NaN.
+// Puts the unit's K largest elements in order and hands (place, key) to `out`, once per place from
+// some lane; places without an element get key 0.  `threshold`: at least k of the unit's elements
+// reach it, or it is -inf or NaN.
 template <int TPU, class SRC, class MEM, class OUT>
 __device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s, float threshold, int k, OUT out) {
   constexpr int kW = TPU / 64, kList = Scratch<TPU>::kList;
@@ -474,29 +518,25 @@ __device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s
     over |= s.count[w] > kList;
   }
   if (over || n > kMaxRanked) {
-    float kv;
-    int ki;
     UnitSync<TPU>();
-    KthElement<TPU>(mem, s.count, floor_v, k, &kv, &ki);
-    UnitSync<TPU>();
-    Collect<TPU>(mem, s, floor_v, [=](float v, int i) { return v > kv || (v == kv && i <= ki); });
+    const uint64_t kth = KthElement<TPU>(mem, s.count, floor_v, k);
+    Collect<TPU>(mem, s, floor_v, [=](float v, int i) { return v >= floor_v && Key(v, i) >= kth; });
     UnitSync<TPU>();
     n = k;
   }
   if (TPU == 64) {
     for (int a = tid; a < n; a += 64) {
-      const Cand mine = s.cand[0][a];
+      const uint64_t mine = s.cand[0][a];
       int place = 0;
 #pragma unroll 4
-      for (int b = 0; b < n; ++b) place += Ahead(s.cand[0][b], mine);
-      if (place < k) out(place, mine.v, mine.i);
+      for (int b = 0; b < n; ++b) place += s.cand[0][b] > mine ? 1 : 0;
+      if (place < k) out(place, mine);
     }
   } else {
     // each wave counts, for every candidate, those of its own list that are ahead
     const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int own_n = s.count[own];
-    for (int a0 = 0; a0 < n; a0 += 64) {
-      const int a = a0 + lane;
+    auto candidate = [&](int a) {  // the a-th of all waves' lists
       int w = 0, i = a;
 #pragma unroll
       for (int x = 0; x < kW - 1; ++x) {
@@ -504,28 +544,20 @@ __device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s
         i = further ? i - s.count[x] : i;
         w = further ? x + 1 : w;
       }
-      if (a < n) {
-        const Cand mine = s.cand[w][i];
-        int place = 0;
+      return s.cand[w][i];
+    };
+    for (int a = lane; a < n; a += 64) {
+      const uint64_t mine = candidate(a);
+      int place = 0;
 #pragma unroll 4
-        for (int b = 0; b < own_n; ++b) place += Ahead(s.cand[own][b], mine);
-        if (place) atomicAdd(&s.place[a], place);
-      }
+      for (int b = 0; b < own_n; ++b) place += s.cand[own][b] > mine ? 1 : 0;
+      if (place) atomicAdd(&s.place[a], place);
     }
     __syncthreads();
-    for (int a = tid; a < n; a += TPU) {
-      if (s.place[a] >= k) continue;
-      int w = 0, i = a;
-#pragma unroll
-      for (int x = 0; x < kW - 1; ++x) {
-        const bool further = w == x && i >= s.count[x];
-        i = further ? i - s.count[x] : i;
-        w = further ? x + 1 : w;
-      }
-      out(s.place[a], s.cand[w][i].v, s.cand[w][i].i);
-    }
+    for (int a = tid; a < n; a += TPU)
+      if (s.place[a] < k) out(s.place[a], candidate(a));
   }
-  for (int a = n + tid; a < k; a += TPU) out(a, -INFINITY, -1);
+  for (int a = n + tid; a < k; a += TPU) out(a, 0);
 }
 
 // ---- scores ------------------------------------------------------------------------------------
@@ -543,8 +575,7 @@ struct ScoresArgs {
   float *logp, *entropy, *stats, *top_v;
   int32_t *top_i;
   Partial *part;       // split rows: [rows][nseg], and [rows][nseg][k] alternatives
-  float *part_v;
-  int32_t *part_i;
+  uint64_t *part_top;
 };
 
 __device__ inline int64_t IdAt(const void *ids, int32_t id64, size_t at) {
@@ -590,12 +621,19 @@ struct TopWriter {
   float *v;
   int32_t *i;
   float base, ls;
-  bool nan;  // the row's sum is NaN (NaN or +inf among its logits): no alternatives
-  __device__ void operator()(int place, float val, int col) const {
-    v[place] = nan ? ls : col < 0 ? -INFINITY : (val - base) - ls;
-    i[place] = nan ? -1 : col;
+  __device__ void operator()(int place, uint64_t key) const {
+    v[place] = key ? (ValueOf(key) - base) - ls : -INFINITY;
+    i[place] = key ? ColumnOf(key) : -1;
   }
 };
+// A row whose sum is NaN (NaN or +inf among its logits) has no alternatives.
+template <int TPU>
+__device__ inline void WriteNoTop(float *v, int32_t *i, float val, int k, int tid) {
+  for (int a = tid; a < k; a += TPU) {
+    v[a] = val;
+    i[a] = -1;
+  }
+}
 
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
 __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a) {
@@ -618,18 +656,20 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
   float cm[NCH], gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
+    cm[c] = -INFINITY;
+    if (!Used<T, TPU>(c, u.n)) continue;
     float half[2] = {T::Get(r[c], 0), T::Get(r[c], 1)};
 #pragma unroll
-    for (int j = 2; j < T::kVec; ++j) half[j & 1] = fmaxf(half[j & 1], T::Get(r[c], j));
-    cm[c] = fmaxf(half[0], half[1]);
+    for (int j = 2; j < T::kVec; ++j) half[j & 1] = Max(half[j & 1], T::Get(r[c], j));
+    cm[c] = Max(half[0], half[1]);
     if (NCH >= 4) {
-      gm[c & 3] = fmaxf(gm[c & 3], cm[c]);
+      gm[c & 3] = Max(gm[c & 3], cm[c]);
     } else {
-      gm[(2 * c) & 3] = fmaxf(gm[(2 * c) & 3], half[0]);
-      gm[(2 * c + 1) & 3] = fmaxf(gm[(2 * c + 1) & 3], half[1]);
+      gm[(2 * c) & 3] = Max(gm[(2 * c) & 3], half[0]);
+      gm[(2 * c + 1) & 3] = Max(gm[(2 * c + 1) & 3], half[1]);
     }
   }
-  const float lane_max = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
+  const float lane_max = Max(Max(gm[0], gm[1]), Max(gm[2], gm[3]));
   if (TOP && TPU > 64) s.group_max[tid] = lane_max;
   const float m = UnitMax<TPU>(lane_max, s.red[0]);
   const float base = Base(m);
@@ -639,6 +679,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
   float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
+    if (!Used<T, TPU>(c, u.n)) continue;
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) {
       const float t = exponent(T::Get(r[c], j)), e = __builtin_amdgcn_exp2f(t);
@@ -668,21 +709,20 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
     WriteRowScores<T>(a, u, x, m, s0, s1);
   }
   if (TOP) {
+    const size_t at = (SPLIT ? static_cast<size_t>(unit) : static_cast<size_t>(u.row)) * a.k;
+    if (isnan(s0)) {  // (the same in all lanes of the unit; split: the joining kernel sees the sum)
+      if (!SPLIT) WriteNoTop<TPU>(a.top_v + at, a.top_i + at, s0, a.k, tid);
+      return;
+    }
     NewPass(r);
     const float threshold = GroupThreshold<TPU>(gm, s, a.k);
     const RegSource<T, NCH, TPU> src{r, cm, u.lo, u.n, tid};
     const MemSource<T, TPU> mem{x + u.lo, u.lo, u.n, tid};
-    const size_t at = (SPLIT ? static_cast<size_t>(unit) : static_cast<size_t>(u.row)) * a.k;
     if (SPLIT) {
-      float *pv = a.part_v + at;
-      int32_t *pi = a.part_i + at;
-      SelectTop<TPU>(src, mem, s, threshold, a.k, [=](int place, float v, int i) {
-        pv[place] = v;
-        pi[place] = i;
-      });
+      uint64_t *list = a.part_top + at;
+      SelectTop<TPU>(src, mem, s, threshold, a.k, [=](int place, uint64_t key) { list[place] = key; });
     } else {
-      const float ls = LogSum(s0);
-      SelectTop<TPU>(src, mem, s, threshold, a.k, TopWriter{a.top_v + at, a.top_i + at, base, ls, isnan(ls)});
+      SelectTop<TPU>(src, mem, s, threshold, a.k, TopWriter{a.top_v + at, a.top_i + at, base, LogSum(s0)});
     }
   }
 }
@@ -691,7 +731,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
 __device__ inline void JoinPartials(const Partial *part, int nseg, float k2, float (*red)[kWaves], float *m_out,
                                     float *s0_out, float *s1_out) {
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < nseg; i += kBlock) m = fmaxf(m, part[i].m);
+  for (int i = threadIdx.x; i < nseg; i += kBlock) m = Max(m, part[i].m);
   m = UnitMax<kBlock>(m, red[0]);
   const float base = Base(m);
   float s0 = 0.0f, s1 = 0.0f;
@@ -727,7 +767,7 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
   }
   const int nseg = a.r.nseg;
   const size_t n = static_cast<size_t>(nseg) * a.k;
-  const ListSource src{a.part_v + u.row * n, a.part_i + u.row * n, static_cast<int>(n), tid};
+  const ListSource src{a.part_top + u.row * n, nseg, a.k, tid};
   if (TOP) {
     float mine = -INFINITY;
     src.Each(0.0f, [&](float v, int) { mine = fmaxf(mine, v); });
@@ -738,13 +778,222 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
   if (tid == 0) WriteRowScores<T>(a, u, x, m, s0, s1);
   if (TOP) {
+    float *tv = a.top_v + static_cast<size_t>(u.row) * a.k;
+    int32_t *ti = a.top_i + static_cast<size_t>(u.row) * a.k;
+    if (isnan(s0)) {
+      WriteNoTop<kBlock>(tv, ti, s0, a.k, tid);
+      return;
+    }
     const float none[4] = {};
     const float threshold = GroupThreshold<kBlock>(none, s, a.k);
-    const float ls = LogSum(s0);
-    SelectTop<kBlock>(src, src, s, threshold, a.k,
-                      TopWriter{a.top_v + static_cast<size_t>(u.row) * a.k, a.top_i + static_cast<size_t>(u.row) * a.k,
-                                Base(m), ls, isnan(ls)});
+    SelectTop<kBlock>(src, src, s, threshold, a.k, TopWriter{tv, ti, Base(m), LogSum(s0)});
   }
+}
+
+// ---- scores of short rows --------------------------------------------------------------------
+// Rows of up to 2 KiB: a wave takes four, 16 lanes (one DPP row) each.  What such a row costs is not
+// its bytes but the steps that are taken once a row -- reductions, threshold, ranking --, and these
+// serve four rows here.
+
+// 16 lanes' values sorted, the largest first: a bitonic sort whose merges start with a mirrored
+// exchange, so that every lane below its partner keeps the larger.
+template <int CTRL>
+__device__ inline float Exchange(float v, bool below) {
+  const float o = Dpp<CTRL>(v, v);
+  return below ? Max(v, o) : Min(v, o);
+}
+__device__ inline float RowSort(float v) {
+  const int l = threadIdx.x & 15;
+  const bool b0 = !(l & 1), b1 = !(l & 2), b2 = !(l & 4), b3 = !(l & 8);
+  v = Exchange<0xb1>(v, b0);   // lane ^ 1
+  v = Exchange<0x1b>(v, b1);   // lane ^ 3
+  v = Exchange<0xb1>(v, b0);
+  v = Exchange<0x141>(v, b2);  // lane ^ 7
+  v = Exchange<0x4e>(v, b1);   // lane ^ 2
+  v = Exchange<0xb1>(v, b0);
+  v = Exchange<0x140>(v, b3);  // lane ^ 15
+  const float up = Dpp<0x104, 0xf, 0x5>(v, v), o = Dpp<0x114, 0xf, 0xa>(up, v);  // lane ^ 4: + 4 or - 4
+  v = b2 ? Max(v, o) : Min(v, o);
+  v = Exchange<0x4e>(v, b1);
+  v = Exchange<0xb1>(v, b0);
+  return v;  // (lane l of the 16: the l-th largest)
+}
+// The k-th largest (k <= 16) of 16 lanes' pairs, in all lanes.
+__device__ inline float RowKthLargest(float a, float b, int k) {
+  const int l = threadIdx.x & 15;
+  a = RowSort(a);
+  b = RowSort(b);
+  // the 16 largest of both: a[l] against b[15 - l], a bitonic sequence that three more exchanges and
+  // the last sort
+  a = Max(a, Dpp<0x140>(b, b));
+  const float x = Dpp<kRowRor + 8>(a, a);  // lane ^ 8
+  a = !(l & 8) ? Max(a, x) : Min(a, x);
+  const float up = Dpp<0x104, 0xf, 0x5>(a, a), o = Dpp<0x114, 0xf, 0xa>(up, a);
+  a = !(l & 4) ? Max(a, o) : Min(a, o);
+  a = Exchange<0x4e>(a, !(l & 2));
+  a = Exchange<0xb1>(a, !(l & 1));
+  return __int_as_float(__builtin_amdgcn_ds_bpermute(((threadIdx.x & 48) + k - 1) * 4, __float_as_int(a)));
+}
+
+constexpr int kShortTop = 16;  // alternatives
+constexpr int kShortCap = 64;  // candidates a row
+
+// KthElement for 16 lanes (a row's lanes are active together or not at all).
+template <class T>
+__device__ __noinline__ uint64_t ShortKthElement(const typename T::Store *p, int n, float floor_v, int k) {
+  const int l = threadIdx.x & 15;
+  auto count = [&](auto pred) {
+    int c = 0;
+    for (int i = l; i < n; i += 16) c += pred(T::Load(p + i), i) ? 1 : 0;
+    return RowSum(c);
+  };
+  uint32_t t = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = t | (1u << bit);
+    if (count([=](float v, int) { return v >= floor_v && OrderKey(v) >= c; }) >= k) t = c;
+  }
+  const float val = KeyValue(t);
+  const int need = k - count([=](float v, int) { return v > val; });
+  int col = 0;
+  for (int bit = 11; bit >= 0; --bit) {  // (columns < 2^11)
+    const int c = col | (1 << bit);
+    if (count([=](float v, int i) { return v == val && i < c; }) < need) col = c;
+  }
+  return Key(val, col);
+}
+// Sum over a row's lanes up to and with one's own.
+__device__ inline int RowPrefix(int v) {
+  v += DppI<0x111>(0, v);  // row_shr:1
+  v += DppI<0x112>(0, v);
+  v += DppI<0x114>(0, v);
+  return v + DppI<0x118>(0, v);
+}
+
+template <class T, int NCH, bool TOP>
+__global__ __launch_bounds__(kBlock) void ScoresShortKernel(const ScoresArgs a) {
+  __shared__ uint64_t lists[TOP ? kBlock / 16 : 1][TOP ? kShortCap : 1];
+  __shared__ uint8_t chunk_lists[TOP ? kBlock / 16 : 1][TOP ? kShortCap : 1];
+  const int l = threadIdx.x & 15;
+  const uint32_t row = blockIdx.x * (kBlock / 16) + (threadIdx.x >> 4);
+  if (row >= a.r.rows) return;
+  const Unit u = GetUnit(a.r, row);
+  if (u.skip) {
+    WriteRowNothing<16>(a, row, l);
+    return;
+  }
+  const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
+  const int n = a.r.vocab;
+  U4 r[NCH];
+  LoadUnit<T, NCH, 16>(x, n, l, r);
+  int64_t tok = -1;
+  float at_tok = 0.0f;
+  if (a.tokens) {
+    tok = IdAt(a.tokens, a.token64, row);
+    if (tok < 0 || tok >= n) tok = -1;
+    if (tok >= 0) at_tok = T::Load(x + tok);
+  }
+  // the maxima of a lane's 16 bytes, and of the even and the odd ones of these
+  float cm[NCH], half[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    cm[c] = -INFINITY;
+    if (!Used<T, 16>(c, n)) continue;
+    cm[c] = T::Get(r[c], 0);
+#pragma unroll
+    for (int j = 1; j < T::kVec; ++j) cm[c] = Max(cm[c], T::Get(r[c], j));
+    half[c & 1] = Max(half[c & 1], cm[c]);
+  }
+  const float lane_max = Max(half[0], half[1]);
+  const float m = RowMax(lane_max), base = Base(m);
+  NewPass(r);
+  const Exponent exponent(base, a.k2);
+  float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    if (!Used<T, 16>(c, n)) continue;
+#pragma unroll
+    for (int j = 0; j < T::kVec; ++j) {
+      const float t = exponent(T::Get(r[c], j)), e = __builtin_amdgcn_exp2f(t);
+      s0 += e;
+      s1 = fmaf(e, fmaxf(t, kLowest), s1);
+    }
+  }
+  s0 = RowSum(s0);
+  s1 = RowSum(s1);
+  const float less = __builtin_amdgcn_exp2f(-exponent.delta);
+  s1 = fmaf(-exponent.delta, s0, s1) * less;
+  s0 *= less;
+  const float ls = LogSum(s0);
+  if (l == 0) {
+    if (a.tokens) a.logp[row] = tok >= 0 ? (at_tok - base) - ls : 0.0f;
+    a.entropy[row] = s0 == 0.0f ? 0.0f : ls - kLn2 * (s1 / s0);
+    *reinterpret_cast<float2 *>(a.stats + 2 * static_cast<size_t>(row)) = float2{m, s0};
+  }
+  if (!TOP) return;
+
+  const int k = a.k;
+  const TopWriter out{a.top_v + static_cast<size_t>(row) * k, a.top_i + static_cast<size_t>(row) * k, base, ls};
+  if (isnan(s0)) {
+    WriteNoTop<16>(out.v, out.i, s0, k, l);
+    return;
+  }
+  // The lane's 16 bytes with a candidate among them, listed; then one lane takes each, from memory
+  // (a register cannot be chosen at run time), and lists its candidates.
+  const float floor_v = Max(RowKthLargest(half[0], half[1], k), kLowest);
+  uint64_t *list = lists[threadIdx.x >> 4];
+  uint32_t hit = 0;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) hit |= cm[c] >= floor_v ? 1u << c : 0u;
+  const int hits = __popc(hit), upto = RowPrefix(hits), listed = RowSum(hits);
+  int count = 0;
+  if (listed <= kShortCap) {
+    uint8_t *chunks = chunk_lists[threadIdx.x >> 4];
+    for (int at = upto - hits; hit; hit &= hit - 1, ++at) chunks[at] = static_cast<uint8_t>((__ffs(hit) - 1) * 16 + l);
+    UnitSync<64>();
+    for (int i = 0; i < listed; i += 16) {  // (mostly once)
+      const bool have = i + l < listed;
+      const int e = (have ? chunks[i + l] : 0) * T::kVec, first = FirstCol<T>(e, n);
+      // (a row of less than 16 bytes: lane 0 has it all)
+      const U4 raw = n >= T::kVec ? *reinterpret_cast<const typename T::Vec *>(x + first) : r[0];
+      uint32_t in = 0;
+#pragma unroll
+      for (int j = 0; j < T::kVec; ++j)
+        in |= have && first + j >= e && T::Get(raw, j) >= floor_v ? 1u << j : 0u;
+      const int some = __popc(in);
+      int at = count + RowPrefix(some) - some;
+#pragma unroll
+      for (int j = 0; j < T::kVec; ++j) {
+        if (in & (1u << j)) {
+          if (at < kShortCap) list[at] = Key(T::Get(raw, j), first + j);
+          ++at;
+        }
+      }
+      count += RowSum(some);
+    }
+  }
+  if (listed > kShortCap || count > kShortCap) {  // many equal values: exactly the k, found by bisection
+    const uint64_t kth = ShortKthElement<T>(x, n, floor_v, k);
+    UnitSync<64>();
+    int pos = 0;
+    for (int i0 = 0; i0 < n; i0 += 16) {
+      const float v = i0 + l < n ? T::Load(x + i0 + l) : -INFINITY;
+      const uint64_t key = Key(v, i0 + l);
+      const int in = v >= floor_v && key >= kth ? 1 : 0;
+      const int upto_me = RowPrefix(in);  // (all of the row's lanes take part)
+      if (in) list[pos + upto_me - 1] = key;
+      pos += RowSum(in);
+    }
+    count = k;
+  }
+  UnitSync<64>();
+  for (int b = l; b < count; b += 16) {
+    const uint64_t mine = list[b];
+    int place = 0;
+#pragma unroll 4
+    for (int o = 0; o < count; ++o) place += list[o] > mine ? 1 : 0;
+    if (place < k) out(place, mine);
+  }
+  for (int b = count + l; b < k; b += 16) out(b, 0);
 }
 
 // ---- gradients -----------------------------------------------------------------------------------
@@ -759,6 +1008,7 @@ template <class T, int NCH, int TPU, class F>
 __device__ inline void StoreUnit(typename T::Store *p, int n, int tid, const U4 (&r)[NCH], F f) {
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
+    if (!Used<T, TPU>(c, n)) continue;
     const int e = (c * TPU + tid) * T::kVec;
     if (e < n) {
       const int first = FirstCol<T>(e, n);
@@ -1011,17 +1261,21 @@ __global__ __launch_bounds__(kThreads<TPU>) void DistillKernel(const DistillArgs
   }
   float m = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+  for (int c = 0; c < NCH; ++c) {
+    if (!Used<T, TPU>(c, u.n)) continue;
 #pragma unroll
-    for (int j = 0; j < T::kVec; ++j) m = fmaxf(m, T::Get(r[c], j));
+    for (int j = 0; j < T::kVec; ++j) m = Max(m, T::Get(r[c], j));
+  }
   m = UnitMax<TPU>(m, list.red[2]);
   NewPass(r);
   const Exponent exponent(Base(m), a.k2);
   float s0 = 0.0f;
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+  for (int c = 0; c < NCH; ++c) {
+    if (!Used<T, TPU>(c, u.n)) continue;
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) s0 += __builtin_amdgcn_exp2f(exponent(T::Get(r[c], j)));
+  }
   s0 = UnitSum<TPU>(s0, list.red[3]) * __builtin_amdgcn_exp2f(-exponent.delta);
   const float ls = LogSum(s0);
   const float loss = Divergence<TPU>(a, t, xs, m, ls, list.red[4]);
@@ -1130,40 +1384,47 @@ int HipFail(const char *what, hipError_t e) {
 }
 
 template <class ARGS>
-int Launch(void (*kernel)(ARGS), uint32_t blocks, const ARGS &args, void *stream) {
+int Launch(void (*kernel)(ARGS), uint32_t blocks, const ARGS &args, void *stream, int threads = kBlock) {
   if (!blocks) return KD_OK;
   void *argv[] = {const_cast<ARGS *>(&args)};
-  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(blocks), dim3(kBlock), argv, 0,
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(blocks), dim3(threads), argv, 0,
                                        static_cast<hipStream_t>(stream));
   return e == hipSuccess ? KD_OK : HipFail("launch", e);
 }
 
 int64_t ElemBytes(int dtype) { return dtype == KD_DTYPE_F32 ? 4 : 2; }
 
-// How rows are dealt out (the comment at the top of this file): TPU threads a unit, NCH 16-byte
+// How rows are dealt out (the comment at the top of this file): TPU threads a unit, up to NCH 16-byte
 // loads each.
 struct Plan {
   int tpu, nch, seg_len, nseg;
 };
-Plan MakePlan(int64_t vocab, int dtype) {
+enum Purpose {
+  kValues,  // statistics, alternatives, losses
+  kFused,   // loss and gradient
+  kPieces,  // a gradient whose statistics are known: any part of a row by itself
+};
+Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what) {
   const int64_t bytes = vocab * ElemBytes(dtype), vec = 16 / ElemBytes(dtype);
-  Plan p;
-  if (bytes <= 8192) {
-    p = {64, 1, static_cast<int>(vocab), 1};
-    while (64 * 16 * p.nch < bytes) p.nch *= 2;
-  } else {
-    const int64_t cap = kBlock * 16 * 8 / ElemBytes(dtype);  // columns of a unit of 32 KiB
-    p.tpu = kBlock;
-    p.nseg = static_cast<int>((vocab + cap - 1) / cap);
-    // equal segments, whole vectors
-    p.seg_len = static_cast<int>(((vocab + p.nseg - 1) / p.nseg + vec - 1) / vec * vec);
-    p.nseg = static_cast<int>((vocab + p.seg_len - 1) / p.seg_len);
-    p.nch = p.seg_len * ElemBytes(dtype) <= kBlock * 16 * 4 ? 4 : 8;
-  }
+  const int whole = static_cast<int>(vocab);
+  if (bytes <= 2048) return {64, 2, whole, 1};
+  if (bytes <= 8192) return {64, 8, whole, 1};
+  if (bytes <= 32768) return {kBlock, 8, whole, 1};
+  if (what != kPieces && bytes <= 65536) return {512, 8, whole, 1};
+  if (what == kFused && bytes <= 131072 && rows >= 32) return {1024, 8, whole, 1};
+  if (what == kFused && bytes <= 262144 && rows >= 128) return {1024, 16, whole, 1};
+  Plan p{kBlock, 8, 0, 0};
+  int64_t cap = 32768;
+  while (cap > 4096 && rows * ((bytes + cap - 1) / cap) < 64) cap /= 2;
+  cap /= ElemBytes(dtype);
+  p.nseg = static_cast<int>((vocab + cap - 1) / cap);
+  // equal segments, whole vectors
+  p.seg_len = static_cast<int>(((vocab + p.nseg - 1) / p.nseg + vec - 1) / vec * vec);
+  p.nseg = static_cast<int>((vocab + p.seg_len - 1) / p.seg_len);
   return p;
 }
 
-int CheckRows(const kd_frame_rows *r, Rows *out, Plan *plan, int64_t *rows) {
+int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64_t *rows) {
   if (!r || r->batch < 0 || r->steps < 0) return SetError(KD_E_INVALID, "bad argument: rows");
   if (r->dtype != KD_DTYPE_F32 && r->dtype != KD_DTYPE_F16 && r->dtype != KD_DTYPE_BF16)
     return SetError(KD_E_INVALID, "bad argument: dtype of the logits");
@@ -1172,9 +1433,9 @@ int CheckRows(const kd_frame_rows *r, Rows *out, Plan *plan, int64_t *rows) {
   if (r->batch > INT32_MAX || r->steps > INT32_MAX || r->batch * r->steps > INT32_MAX)
     return SetError(KD_E_INVALID, "bad argument: more than 2^31 - 1 rows");
   *rows = r->batch * r->steps;
-  *plan = MakePlan(r->vocab, r->dtype);
+  *plan = MakePlan(r->vocab, r->dtype, *rows, what);
   // (a grid has fewer than 2^32 threads)
-  if (*rows * plan->nseg > ((int64_t(1) << 24) - 1) * (kBlock / plan->tpu))
+  if (*rows * plan->nseg > ((int64_t(1) << 32) - 1) / plan->tpu)
     return SetError(KD_E_INVALID, "bad argument: rows x vocab is too large for one call");
   if (r->batch_stride < 0 || r->row_stride < 0) return SetError(KD_E_INVALID, "bad argument: negative stride");
   if (*rows && !r->logits) return SetError(KD_E_INVALID, "bad argument: logits is NULL");
@@ -1225,17 +1486,14 @@ template <int N>
 struct Int {
   static constexpr int value = N;
 };
-template <class T, class F>
+template <Purpose WHAT, class T, class F>
 int ForPlan(const Plan &p, F f) {
-  if (p.tpu == 64) {
-    switch (p.nch) {
-      case 1: return f(T{}, Int<1>{}, Int<64>{});
-      case 2: return f(T{}, Int<2>{}, Int<64>{});
-      case 4: return f(T{}, Int<4>{}, Int<64>{});
-      default: return f(T{}, Int<8>{}, Int<64>{});
-    }
-  }
-  return p.nch == 4 ? f(T{}, Int<4>{}, Int<kBlock>{}) : f(T{}, Int<8>{}, Int<kBlock>{});
+  if (p.tpu == 64) return p.nch == 2 ? f(T{}, Int<2>{}, Int<64>{}) : f(T{}, Int<8>{}, Int<64>{});
+  if constexpr (WHAT != kPieces)
+    if (p.tpu == 512) return f(T{}, Int<8>{}, Int<512>{});
+  if constexpr (WHAT == kFused)
+    if (p.tpu == 1024) return p.nch == 8 ? f(T{}, Int<8>{}, Int<1024>{}) : f(T{}, Int<16>{}, Int<1024>{});
+  return f(T{}, Int<8>{}, Int<kBlock>{});
 }
 template <class F>
 int ForType(int dtype, F f) {
@@ -1259,14 +1517,27 @@ int LaunchScores(const kd_frame_rows *rows, const ScoresArgs &a, const Plan &pla
   return ForType(rows->dtype, [&](auto t) {
     using T = decltype(t);
     if constexpr (SPLIT) {
-      return plan.nch == 4 ? Launch(ScoresKernel<T, 4, kBlock, true, ENT, TOP>, Blocks(a.r, plan), a, stream)
-                           : Launch(ScoresKernel<T, 8, kBlock, true, ENT, TOP>, Blocks(a.r, plan), a, stream);
+      return Launch(ScoresKernel<T, 8, kBlock, true, ENT, TOP>, Blocks(a.r, plan), a, stream);
     } else {
-      return ForPlan<T>(plan, [&](auto tt, auto nch, auto tpu) {
+      return ForPlan<kValues, T>(plan, [&](auto tt, auto nch, auto tpu) {
         return Launch(ScoresKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value, false, ENT, TOP>,
-                      Blocks(a.r, plan), a, stream);
+                      Blocks(a.r, plan), a, stream, kThreads<decltype(tpu)::value>);
       });
     }
+  });
+}
+
+bool IsShort(int64_t vocab, int dtype) { return vocab * ElemBytes(dtype) <= 16 * 16 * 8; }
+template <bool TOP>
+int LaunchShort(const kd_frame_rows *rows, const ScoresArgs &a, void *stream) {
+  const uint32_t blocks = (a.r.rows + kBlock / 16 - 1) / (kBlock / 16);
+  const int64_t bytes = rows->vocab * ElemBytes(rows->dtype);
+  return ForType(rows->dtype, [&](auto t) {
+    using T = decltype(t);
+    return bytes <= 256    ? Launch(ScoresShortKernel<T, 1, TOP>, blocks, a, stream)
+           : bytes <= 512  ? Launch(ScoresShortKernel<T, 2, TOP>, blocks, a, stream)
+           : bytes <= 1024 ? Launch(ScoresShortKernel<T, 4, TOP>, blocks, a, stream)
+                           : Launch(ScoresShortKernel<T, 8, TOP>, blocks, a, stream);
   });
 }
 
@@ -1278,9 +1549,9 @@ size_t kd_token_scores_workspace(const kd_frame_rows *rows, int32_t top) {
   Rows r;
   Plan p;
   int64_t n;
-  if (CheckRows(rows, &r, &p, &n) || top < 0 || top > kMaxTop || p.nseg == 1) return 0;
+  if (CheckRows(rows, kValues, &r, &p, &n) || top < 0 || top > kMaxTop || p.nseg == 1) return 0;
   const size_t units = static_cast<size_t>(n) * p.nseg;
-  return Align(units * sizeof(Partial)) + (top ? Align(units * top * 4) * 2 : 0);
+  return Align(units * sizeof(Partial)) + units * top * sizeof(uint64_t);
 }
 
 int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token_bytes, int32_t top, float *logp,
@@ -1290,7 +1561,7 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
     ScoresArgs a{};
     Plan p;
     int64_t n;
-    if (int rc = CheckRows(rows, &a.r, &p, &n)) return rc;
+    if (int rc = CheckRows(rows, kValues, &a.r, &p, &n)) return rc;
     if (top < 0 || top > kMaxTop) return SetError(KD_E_INVALID, "bad argument: top must be between 0 and 64");
     if (tokens && token_bytes != 4 && token_bytes != 8)
       return SetError(KD_E_INVALID, "bad argument: token_bytes must be 4 or 8");
@@ -1311,14 +1582,16 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
     a.top_i = top_ids;
     DeviceGuard guard(rows->device);
     if (guard.error() != hipSuccess) return HipFail("hipSetDevice", guard.error());
+    // Short rows, four to a wave; more than 16 alternatives need the 64 groups of a whole wave.
+    if (IsShort(a.r.vocab, rows->dtype) && top <= kShortTop)
+      return top ? LaunchShort<true>(rows, a, stream) : LaunchShort<false>(rows, a, stream);
     if (p.nseg == 1)
       return top ? LaunchScores<false, true, true>(rows, a, p, stream)
                  : LaunchScores<false, true, false>(rows, a, p, stream);
     const size_t units = static_cast<size_t>(n) * p.nseg;
     char *ws = static_cast<char *>(workspace);
     a.part = reinterpret_cast<Partial *>(ws);
-    a.part_v = reinterpret_cast<float *>(ws + Align(units * sizeof(Partial)));
-    a.part_i = reinterpret_cast<int32_t *>(ws + Align(units * sizeof(Partial)) + Align(units * top * 4));
+    a.part_top = reinterpret_cast<uint64_t *>(ws + Align(units * sizeof(Partial)));
     if (int rc = top ? LaunchScores<true, true, true>(rows, a, p, stream)
                      : LaunchScores<true, true, false>(rows, a, p, stream))
       return rc;
@@ -1337,7 +1610,7 @@ int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t 
     ScoresGradArgs a{};
     Plan p;
     int64_t n;
-    if (int rc = CheckRows(rows, &a.r, &p, &n)) return rc;
+    if (int rc = CheckRows(rows, kPieces, &a.r, &p, &n)) return rc;
     if (tokens && token_bytes != 4 && token_bytes != 8)
       return SetError(KD_E_INVALID, "bad argument: token_bytes must be 4 or 8");
     if (!n) return KD_OK;
@@ -1352,19 +1625,19 @@ int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t 
     DeviceGuard guard(rows->device);
     if (guard.error() != hipSuccess) return HipFail("hipSetDevice", guard.error());
     return ForType(rows->dtype, [&](auto t) {
-      return ForPlan<decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+      return ForPlan<kPieces, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
         return Launch(ScoresGradKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value>, Blocks(a.r, p), a,
-                      stream);
+                      stream, kThreads<decltype(tpu)::value>);
       });
     });
   });
 }
 
-size_t kd_distill_loss_workspace(const kd_frame_rows *rows) {
+size_t kd_distill_loss_workspace(const kd_frame_rows *rows, int32_t with_grad) {
   Rows r;
   Plan p;
   int64_t n;
-  if (CheckRows(rows, &r, &p, &n) || p.nseg == 1) return 0;
+  if (CheckRows(rows, with_grad ? kFused : kValues, &r, &p, &n) || p.nseg == 1) return 0;
   return Align(static_cast<size_t>(n) * p.nseg * sizeof(Partial)) + Align(static_cast<size_t>(n) * 8);
 }
 
@@ -1375,7 +1648,9 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
     DistillArgs a{};
     Plan p;
     int64_t n;
-    if (int rc = CheckRows(rows, &a.r, &p, &n)) return rc;
+    // stats given and no loss asked for: the statistics of an earlier call, the gradient alone
+    const bool known = !loss && stats;
+    if (int rc = CheckRows(rows, known ? kPieces : grad ? kFused : kValues, &a.r, &p, &n)) return rc;
     if (!teacher || teacher->slots < 1 || teacher->slots > kMaxSlots)
       return SetError(KD_E_INVALID, "bad argument: a teacher lists between 1 and 256 tokens a row");
     if (teacher->id_bytes != 4 && teacher->id_bytes != 8)
@@ -1387,12 +1662,10 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
     if (!n) return KD_OK;
     if (!teacher->ids || !teacher->logits) return SetError(KD_E_INVALID, "bad argument: the teacher's list is NULL");
     if (!loss && !grad) return SetError(KD_E_INVALID, "bad argument: neither loss nor gradient asked for");
-    // stats given and no loss asked for: the statistics of an earlier call, the gradient alone
-    const bool known = !loss && stats;
     if (!loss && !stats) return SetError(KD_E_INVALID, "bad argument: a gradient alone needs the loss's stats");
     if (grad)
       if (int rc = CheckGrad(rows, grad, grad_batch_stride, grad_row_stride, &a.o)) return rc;
-    const size_t need = known ? 0 : kd_distill_loss_workspace(rows);
+    const size_t need = known ? 0 : kd_distill_loss_workspace(rows, grad != nullptr);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
       return SetError(KD_E_INVALID, "bad argument: the workspace is too small (kd_distill_loss_workspace) or unaligned");
     a.ids = teacher->ids;
@@ -1426,18 +1699,23 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
     }
     if (p.nseg > 1 || known) {
       return ForType(rows->dtype, [&](auto t) {
-        return ForPlan<decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+        return ForPlan<kPieces, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
           return Launch(DistillGradKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value>, Blocks(a.r, p), a,
                         stream);
         });
       });
     }
     return ForType(rows->dtype, [&](auto t) {
-      return ForPlan<decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
-        using T = decltype(tt);
-        constexpr int N = decltype(nch)::value, TPU = decltype(tpu)::value;
-        return grad ? Launch(DistillKernel<T, N, TPU, true>, Blocks(a.r, p), a, stream)
-                    : Launch(DistillKernel<T, N, TPU, false>, Blocks(a.r, p), a, stream);
+      if (grad)
+        return ForPlan<kFused, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+          constexpr int TPU = decltype(tpu)::value;
+          return Launch(DistillKernel<decltype(tt), decltype(nch)::value, TPU, true>, Blocks(a.r, p), a, stream,
+                        kThreads<TPU>);
+        });
+      return ForPlan<kValues, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+        constexpr int TPU = decltype(tpu)::value;
+        return Launch(DistillKernel<decltype(tt), decltype(nch)::value, TPU, false>, Blocks(a.r, p), a, stream,
+                      kThreads<TPU>);
       });
     });
   });

@@ -253,7 +253,7 @@ std::pair<Tensor, Tensor> Distill(const Tensor &x, const Tensor &ids, const Tens
     rs = dx.stride(-2);
   }
   Join(rows.r, want_grad ? &bs : nullptr, rs);
-  const size_t bytes = want_loss ? kd_distill_loss_workspace(&rows.r) : 0;
+  const size_t bytes = want_loss ? kd_distill_loss_workspace(&rows.r, want_grad) : 0;
   const Tensor ws = Workspace(bytes, x);
   kd_teacher_rows t{};
   t.ids = id.data_ptr();

@@ -163,7 +163,7 @@ def lib():
     L.kd_token_scores_workspace.restype = C.c_size_t
     L.kd_token_scores.argtypes = [rows, ptr, C.c_int32, C.c_int32, ptr, ptr, ptr, ptr, ptr, ptr, C.c_size_t, ptr]
     L.kd_token_scores_grad.argtypes = [rows, ptr, C.c_int32, ptr, ptr, ptr, ptr, ptr, C.c_int64, C.c_int64, ptr]
-    L.kd_distill_loss_workspace.argtypes = [rows]
+    L.kd_distill_loss_workspace.argtypes = [rows, C.c_int32]
     L.kd_distill_loss_workspace.restype = C.c_size_t
     L.kd_distill_loss.argtypes = [rows, C.POINTER(TeacherRows), ptr, C.c_float, ptr, ptr, ptr, ptr, C.c_int64,
                                   C.c_int64, ptr, C.c_size_t, ptr]

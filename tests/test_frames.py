@@ -33,7 +33,7 @@ def test_rows_that_the_entries_refuse(bad, text):
     _refused(L.kd_token_scores(r, None, 0, 0, None, one, one, None, None, None, 0, None), text)
     _refused(L.kd_token_scores_grad(r, None, 0, one, one, None, None, one, 0, 10, None), text)
     _refused(L.kd_distill_loss(r, C.byref(t), None, 1.0, one, None, None, None, 0, 0, None, 0, None), text)
-    assert L.kd_token_scores_workspace(r, 0) == 0 and L.kd_distill_loss_workspace(r) == 0
+    assert L.kd_token_scores_workspace(r, 0) == 0 and L.kd_distill_loss_workspace(r, 1) == 0
 
 
 def test_arguments_that_the_entries_refuse():
