@@ -317,8 +317,7 @@ struct Exponent {
 // ---- the K largest -------------------------------------------------------------------------------
 // Order: larger value first, then lower column.  -inf and NaN are no candidates.
 //
-// 1. A threshold: about the K-th largest of the maxima of 256 (a wave's unit: 64 or 256) groups of
-//    the unit's elements: at least K elements reach it, and of data in no particular order few more.
+// 1. A threshold from the maxima of 64 or 128 groups of the unit's elements.
 // 2. The elements that reach it are collected in LDS, each wave's in a list of its own.  Where they
 //    are more than the lists hold (many equal values, or most of the large ones in few groups) the
 //    K-th element itself is found by bisection, its value bit by bit and then, among equals, its
@@ -356,42 +355,70 @@ __device__ inline uint64_t Key(float v, int col) {
 __device__ inline float ValueOf(uint64_t key) { return KeyValue(static_cast<uint32_t>(key >> 32)); }
 __device__ inline int ColumnOf(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
 
-// A value that at least k (<= 64 * G) of a wave's 64 * G values reach, and few more than k do: the
-// upper half of the k-th largest's key, bit by bit.
-template <int G>
-__device__ inline float KthLargest(const float (&v)[G], int k) {
-  uint32_t key[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) key[g] = OrderKey(v[g]);
-  uint32_t t = 0;
-  for (int bit = 31; bit >= 16; --bit) {
-    const uint32_t c = t | (1u << bit);
-    int n = 0;
-#pragma unroll
-    for (int g = 0; g < G; ++g) n += Popc(__ballot(key[g] >= c));
-    if (n >= k) {
-      t = c;
-      if (n == k) break;
-    }
-  }
-  // (a key below that of -inf is a NaN's; SelectTop takes either for "all")
-  return KeyValue(t);
+// Values sorted over lanes, the largest first: bitonic sorts whose merges start with a mirrored
+// exchange, so that every lane below its partner keeps the larger.
+__device__ inline float Keep(float v, float o, bool below) { return below ? Max(v, o) : Min(v, o); }
+template <int CTRL>
+__device__ inline float Exchange(float v, bool below) {
+  return Keep(v, Dpp<CTRL>(v, v), below);
 }
-// The same of a unit's group maxima: a lane's own in a unit of one wave, else those in LDS -- by one
-// wave, while the others' issue slots are free for other units (by each wave: 12.2 instead of 10.6 us
-// where a unit of four waves takes a row of 5003 columns).
-template <int TPU>
-__device__ inline float GroupThreshold(const float (&gm)[4], Scratch<TPU> &s, int k) {
-  if (TPU == 64) {
-    if (k > 16) return KthLargest<4>(gm, k);
-    const float g[1] = {Max(Max(gm[0], gm[1]), Max(gm[2], gm[3]))};
-    return KthLargest<1>(g, k);
+__device__ inline float Exchange4(float v) {  // lane ^ 4: the lane 4 further or 4 before
+  const float up = Dpp<0x104, 0xf, 0x5>(v, v);
+  return Keep(v, Dpp<0x114, 0xf, 0xa>(up, v), !(threadIdx.x & 4));
+}
+__device__ inline float RowMerge8(float v) {  // 8 lanes' bitonic sequences
+  const int l = threadIdx.x;
+  v = Exchange4(v);
+  v = Exchange<0x4e>(v, !(l & 2));  // lane ^ 2
+  return Exchange<0xb1>(v, !(l & 1));
+}
+__device__ inline float RowMerge(float v) {  // 16 lanes'
+  return RowMerge8(Exchange<kRowRor + 8>(v, !(threadIdx.x & 8)));
+}
+__device__ inline float RowSort(float v) {  // 16 lanes
+  const int l = threadIdx.x;
+  const bool b0 = !(l & 1), b1 = !(l & 2);
+  v = Exchange<0xb1>(v, b0);
+  v = Exchange<0x1b>(v, b1);  // lane ^ 3
+  v = Exchange<0xb1>(v, b0);
+  v = Exchange<0x141>(v, !(l & 4));  // lane ^ 7
+  v = Exchange<0x4e>(v, b1);
+  v = Exchange<0xb1>(v, b0);
+  return RowMerge8(Exchange<0x140>(v, !(l & 8)));  // lane ^ 15
+}
+__device__ inline float OfLane(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_ds_bpermute(lane * 4, __float_as_int(v)));
+}
+__device__ inline float WaveSort(float v) {
+  const int l = threadIdx.x & 63;
+  v = RowSort(v);
+  v = RowMerge(Keep(v, OfLane(v, l ^ 31), !(l & 16)));
+  v = Keep(v, OfLane(v, l ^ 63), !(l & 32));
+  return RowMerge(Keep(v, OfLane(v, l ^ 16), !(l & 16)));
+}
+
+// A value that at least k of a unit's elements reach, and few more than k do: about the k-th largest
+// of the maxima of 64 groups of them (k <= 32; candidates of data in no particular order: 24 for 20)
+// or of 128 (the 64th; 89 for 64).  `g`: a unit of one wave has its groups' maxima in its lanes; else
+// they are in LDS, and one wave sorts while the others' issue slots are free for other units.
+__device__ inline float WaveThreshold(float a, float b, int k) {
+  if (k <= 32) {
+    const float v = WaveSort(Max(a, b));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1));
   }
+  a = WaveSort(a);
+  b = WaveSort(b);
+  // the 64 largest of both are the larger of the l-th and the (63 - l)-th
+  return -WaveMax(-Max(a, OfLane(b, (threadIdx.x & 63) ^ 63)));
+}
+template <int TPU>
+__device__ inline float GroupThreshold(const float (&g)[2], Scratch<TPU> &s, int k) {
+  if (TPU == 64) return WaveThreshold(g[0], g[1], k);
   if (threadIdx.x < 64) {
-    float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    float m[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int w = 0; w < TPU / 64; ++w) g[w & 3] = Max(g[w & 3], s.group_max[64 * w + threadIdx.x]);
-    const float t = KthLargest<4>(g, k);
+    for (int w = 0; w < TPU / 64; ++w) m[w & 1] = Max(m[w & 1], s.group_max[64 * w + threadIdx.x]);
+    const float t = WaveThreshold(m[0], m[1], k);
     if (threadIdx.x == 0) s.threshold = t;
   }
   __syncthreads();
@@ -455,6 +482,31 @@ struct ListSource {
   }
 };
 
+// The same list in registers.
+template <int N>
+struct HeldSource {
+  uint64_t key[N];
+  __device__ void Load(const ListSource &l) {
+    int at = l.tid / l.nseg, seg = l.tid - at * l.nseg;
+    const int ats = kBlock / l.nseg, segs = kBlock - ats * l.nseg;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      key[i] = at < l.k ? l.list[static_cast<size_t>(seg) * l.k + at] : 0;
+      at += ats;
+      seg += segs;
+      if (seg >= l.nseg) {
+        seg -= l.nseg;
+        ++at;
+      }
+    }
+  }
+  template <class F>
+  __device__ void Each(float, F f) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f(ValueOf(key[i]), ColumnOf(key[i]));
+  }
+};
+
 // Collects a wave's elements that `pred` holds for (none below floor_v); their number, kept or not,
 // in s.count[wave].
 template <int TPU, class SRC, class PRED>
@@ -510,20 +562,24 @@ __device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s
   if (TPU > 64)
     for (int a = tid; a < kMaxRanked; a += TPU) s.place[a] = 0;
   UnitSync<TPU>();
-  int n = 0;
-  bool over = false;
+  int end[kW];  // of the waves' lists, one after the other
+  auto count = [&] {
+    bool over = false;
 #pragma unroll
-  for (int w = 0; w < kW; ++w) {
-    n += s.count[w];
-    over |= s.count[w] > kList;
-  }
-  if (over || n > kMaxRanked) {
+    for (int w = 0; w < kW; ++w) {
+      end[w] = s.count[w] + (w ? end[w - 1] : 0);
+      over |= s.count[w] > kList;
+    }
+    return over || end[kW - 1] > kMaxRanked;
+  };
+  if (count()) {
     UnitSync<TPU>();
     const uint64_t kth = KthElement<TPU>(mem, s.count, floor_v, k);
     Collect<TPU>(mem, s, floor_v, [=](float v, int i) { return v >= floor_v && Key(v, i) >= kth; });
     UnitSync<TPU>();
-    n = k;
+    count();
   }
+  const int n = end[kW - 1];
   if (TPU == 64) {
     for (int a = tid; a < n; a += 64) {
       const uint64_t mine = s.cand[0][a];
@@ -537,25 +593,35 @@ __device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s
     const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int own_n = s.count[own];
     auto candidate = [&](int a) {  // the a-th of all waves' lists
-      int w = 0, i = a;
+      int w = 0, first = 0;
 #pragma unroll
       for (int x = 0; x < kW - 1; ++x) {
-        const bool further = w == x && i >= s.count[x];
-        i = further ? i - s.count[x] : i;
-        w = further ? x + 1 : w;
+        w = a >= end[x] ? x + 1 : w;
+        first = a >= end[x] ? end[x] : first;
       }
-      return s.cand[w][i];
+      return s.cand[w][a - first];
     };
-    for (int a = lane; a < n; a += 64) {
-      const uint64_t mine = candidate(a);
+    auto ahead = [&](uint64_t mine) {
       int place = 0;
 #pragma unroll 4
       for (int b = 0; b < own_n; ++b) place += s.cand[own][b] > mine ? 1 : 0;
-      if (place) atomicAdd(&s.place[a], place);
+      return place;
+    };
+    if (n <= 64) {  // (nearly always, up to 32 alternatives: a candidate a lane)
+      const uint64_t mine = lane < n ? candidate(lane) : 0;
+      const int place = ahead(mine);
+      if (place && lane < n) atomicAdd(&s.place[lane], place);
+      __syncthreads();
+      if (tid < n && s.place[tid] < k) out(s.place[tid], mine);
+    } else {
+      for (int a = lane; a < n; a += 64) {
+        const int place = ahead(candidate(a));
+        if (place) atomicAdd(&s.place[a], place);
+      }
+      __syncthreads();
+      for (int a = tid; a < n; a += TPU)
+        if (s.place[a] < k) out(s.place[a], candidate(a));
     }
-    __syncthreads();
-    for (int a = tid; a < n; a += TPU)
-      if (s.place[a] < k) out(s.place[a], candidate(a));
   }
   for (int a = n + tid; a < k; a += TPU) out(a, 0);
 }
@@ -582,6 +648,18 @@ __device__ inline int64_t IdAt(const void *ids, int32_t id64, size_t at) {
   return id64 ? static_cast<const int64_t *>(ids)[at] : static_cast<const int32_t *>(ids)[at];
 }
 
+// The row's token's logit: two loads that depend on each other, so they are issued with the row's own.
+struct TokenLogit {
+  bool there;
+  float x;
+};
+template <class T>
+__device__ inline TokenLogit LoadToken(const ScoresArgs &a, uint32_t row, const typename T::Store *x) {
+  const int64_t tok = a.tokens ? IdAt(a.tokens, a.token64, row) : -1;
+  const bool there = tok >= 0 && tok < a.r.vocab;
+  return {there, there ? T::Load(x + tok) : 0.0f};
+}
+
 // A row's statistics are its maximum m and s = sum e_j.  (Not log s: 1 / s is what the gradient
 // multiplies by, and a rounded log s of 10 would cost it 3 bits.)  A row without a finite value has
 // m = -inf and s = 0; what is taken relative to its maximum is then taken relative to Base(m) = 0.
@@ -589,17 +667,12 @@ __device__ inline float Base(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ inline float LogSum(float s0) { return s0 == 0.0f ? 0.0f : logf(s0); }
 
 // s1 = sum e_j log2(e_j): H = log s - ln 2 s1 / s, two terms that are at least 0: nothing cancels.
-template <class T>
-__device__ inline void WriteRowScores(const ScoresArgs &a, const Unit &u, const typename T::Store *x, float m,
-                                      float s0, float s1) {
+__device__ inline void WriteRowScores(const ScoresArgs &a, uint32_t row, TokenLogit tok, float m, float s0, float s1) {
   const float ls = LogSum(s0);
-  if (a.tokens) {
-    const int64_t tok = IdAt(a.tokens, a.token64, u.row);
-    a.logp[u.row] = tok >= 0 && tok < a.r.vocab ? (T::Load(x + tok) - Base(m)) - ls : 0.0f;
-  }
-  a.entropy[u.row] = s0 == 0.0f ? 0.0f : ls - kLn2 * (s1 / s0);
-  a.stats[2 * static_cast<size_t>(u.row)] = m;
-  a.stats[2 * static_cast<size_t>(u.row) + 1] = s0;
+  if (a.tokens) a.logp[row] = tok.there ? (tok.x - Base(m)) - ls : 0.0f;
+  a.entropy[row] = s0 == 0.0f ? 0.0f : ls - kLn2 * (s1 / s0);
+  a.stats[2 * static_cast<size_t>(row)] = m;
+  a.stats[2 * static_cast<size_t>(row) + 1] = s0;
 }
 
 // Rows that are not read: zeros, and no alternatives.
@@ -651,9 +724,11 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
   U4 r[NCH];
   LoadUnit<T, NCH, TPU>(x + u.lo, u.n, tid, r);
+  TokenLogit tok{false, 0.0f};
+  if (!SPLIT) tok = LoadToken<T>(a, u.row, x);
 
-  // the maxima of a lane's 16 bytes, of four groups of its elements, and of all of them
-  float cm[NCH], gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  // the maxima of a lane's 16 bytes, of its even and its odd columns, and of all
+  float cm[NCH], g[2] = {-INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     cm[c] = -INFINITY;
@@ -662,14 +737,10 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
 #pragma unroll
     for (int j = 2; j < T::kVec; ++j) half[j & 1] = Max(half[j & 1], T::Get(r[c], j));
     cm[c] = Max(half[0], half[1]);
-    if (NCH >= 4) {
-      gm[c & 3] = Max(gm[c & 3], cm[c]);
-    } else {
-      gm[(2 * c) & 3] = Max(gm[(2 * c) & 3], half[0]);
-      gm[(2 * c + 1) & 3] = Max(gm[(2 * c + 1) & 3], half[1]);
-    }
+    g[0] = Max(g[0], half[0]);
+    g[1] = Max(g[1], half[1]);
   }
-  const float lane_max = Max(Max(gm[0], gm[1]), Max(gm[2], gm[3]));
+  const float lane_max = Max(g[0], g[1]);
   if (TOP && TPU > 64) s.group_max[tid] = lane_max;
   const float m = UnitMax<TPU>(lane_max, s.red[0]);
   const float base = Base(m);
@@ -706,7 +777,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
   if (SPLIT) {
     if (tid == 0) a.part[unit] = Partial{m, s0, s1, 0.0f};
   } else if (tid == 0) {
-    WriteRowScores<T>(a, u, x, m, s0, s1);
+    WriteRowScores(a, u.row, tok, m, s0, s1);
   }
   if (TOP) {
     const size_t at = (SPLIT ? static_cast<size_t>(unit) : static_cast<size_t>(u.row)) * a.k;
@@ -715,7 +786,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
       return;
     }
     NewPass(r);
-    const float threshold = GroupThreshold<TPU>(gm, s, a.k);
+    const float threshold = GroupThreshold<TPU>(g, s, a.k);
     const RegSource<T, NCH, TPU> src{r, cm, u.lo, u.n, tid};
     const MemSource<T, TPU> mem{x + u.lo, u.lo, u.n, tid};
     if (SPLIT) {
@@ -727,23 +798,28 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
   }
 }
 
-// A row's statistics from its segments' (the whole workgroup).
-__device__ inline void JoinPartials(const Partial *part, int nseg, float k2, float (*red)[kWaves], float *m_out,
-                                    float *s0_out, float *s1_out) {
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < nseg; i += kBlock) m = Max(m, part[i].m);
+// A row's statistics from its segments' (the whole workgroup).  `mine`: the thread's first part, loaded
+// before (or one that adds nothing).
+__device__ inline Partial FirstPartial(const Partial *part, int nseg) {
+  return static_cast<int>(threadIdx.x) < nseg ? part[threadIdx.x] : Partial{-INFINITY, 0.0f, 0.0f, 0.0f};
+}
+__device__ inline void JoinPartials(const Partial *part, Partial mine, int nseg, float k2, float (*red)[kWaves],
+                                    float *m_out, float *s0_out, float *s1_out) {
+  float m = mine.m;
+  for (int i = threadIdx.x + kBlock; i < nseg; i += kBlock) m = Max(m, part[i].m);
   m = UnitMax<kBlock>(m, red[0]);
   const float base = Base(m);
   float s0 = 0.0f, s1 = 0.0f;
-  for (int i = threadIdx.x; i < nseg; i += kBlock) {
-    const Partial p = part[i];
+  auto add = [&](const Partial &p) {
     const float t = (Base(p.m) - base) * k2, f = __builtin_amdgcn_exp2f(t);
     // (a segment that adds nothing may have any maximum: its products are not formed)
     if (f != 0.0f && p.s0 != 0.0f) {
       s0 = fmaf(f, p.s0, s0);
       s1 += f * fmaf(t, p.s0, p.s1);
     }
-  }
+  };
+  add(mine);
+  for (int i = threadIdx.x + kBlock; i < nseg; i += kBlock) add(part[i]);
   s0 = WaveSum(s0);
   s1 = WaveSum(s1);
   if ((threadIdx.x & 63) == 0) {
@@ -756,6 +832,9 @@ __device__ inline void JoinPartials(const Partial *part, int nseg, float k2, flo
   *s1_out = SumOf<kBlock>(red[2]);
 }
 
+// One workgroup a row.  It is as long as the loads that wait for each other, so the parts, the token's
+// logit and (up to kHeld a thread) the lists are all loaded at once.
+constexpr int kHeld = 8;
 template <class T, bool TOP>
 __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
   __shared__ Scratch<kBlock> s;
@@ -765,28 +844,42 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
     WriteRowNothing<kBlock>(a, u.row, tid);
     return;
   }
-  const int nseg = a.r.nseg;
-  const size_t n = static_cast<size_t>(nseg) * a.k;
-  const ListSource src{a.part_top + u.row * n, nseg, a.k, tid};
+  const int nseg = a.r.nseg, k = a.k;
+  const Partial *part = a.part + static_cast<size_t>(u.row) * nseg;
+  const Partial mine = FirstPartial(part, nseg);
+  const ListSource list{a.part_top + static_cast<size_t>(u.row) * nseg * k, nseg, k, tid};
+  HeldSource<kHeld> held;
+  const bool hold = nseg * k <= kHeld * kBlock;
+  if (TOP && hold) held.Load(list);
+  const TokenLogit tok = LoadToken<T>(a, u.row, RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u));
   if (TOP) {
-    float mine = -INFINITY;
-    src.Each(0.0f, [&](float v, int) { mine = fmaxf(mine, v); });
-    s.group_max[tid] = mine;
+    float most = -INFINITY;
+    auto more = [&](float v, int) { most = fmaxf(most, v); };
+    if (hold) {
+      held.Each(0.0f, more);
+    } else {
+      list.Each(0.0f, more);
+    }
+    s.group_max[tid] = most;
   }
   float m, s0, s1;
-  JoinPartials(a.part + static_cast<size_t>(u.row) * nseg, nseg, a.k2, s.red, &m, &s0, &s1);
-  const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
-  if (tid == 0) WriteRowScores<T>(a, u, x, m, s0, s1);
+  JoinPartials(part, mine, nseg, a.k2, s.red, &m, &s0, &s1);
+  if (tid == 0) WriteRowScores(a, u.row, tok, m, s0, s1);
   if (TOP) {
-    float *tv = a.top_v + static_cast<size_t>(u.row) * a.k;
-    int32_t *ti = a.top_i + static_cast<size_t>(u.row) * a.k;
+    float *tv = a.top_v + static_cast<size_t>(u.row) * k;
+    int32_t *ti = a.top_i + static_cast<size_t>(u.row) * k;
     if (isnan(s0)) {
-      WriteNoTop<kBlock>(tv, ti, s0, a.k, tid);
+      WriteNoTop<kBlock>(tv, ti, s0, k, tid);
       return;
     }
-    const float none[4] = {};
-    const float threshold = GroupThreshold<kBlock>(none, s, a.k);
-    SelectTop<kBlock>(src, src, s, threshold, a.k, TopWriter{tv, ti, Base(m), LogSum(s0)});
+    const float none[2] = {};
+    const float threshold = GroupThreshold<kBlock>(none, s, k);
+    const TopWriter out{tv, ti, Base(m), LogSum(s0)};
+    if (hold) {
+      SelectTop<kBlock>(held, list, s, threshold, k, out);
+    } else {
+      SelectTop<kBlock>(list, list, s, threshold, k, out);
+    }
   }
 }
 
@@ -795,44 +888,13 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
 // its bytes but the steps that are taken once a row -- reductions, threshold, ranking --, and these
 // serve four rows here.
 
-// 16 lanes' values sorted, the largest first: a bitonic sort whose merges start with a mirrored
-// exchange, so that every lane below its partner keeps the larger.
-template <int CTRL>
-__device__ inline float Exchange(float v, bool below) {
-  const float o = Dpp<CTRL>(v, v);
-  return below ? Max(v, o) : Min(v, o);
-}
-__device__ inline float RowSort(float v) {
-  const int l = threadIdx.x & 15;
-  const bool b0 = !(l & 1), b1 = !(l & 2), b2 = !(l & 4), b3 = !(l & 8);
-  v = Exchange<0xb1>(v, b0);   // lane ^ 1
-  v = Exchange<0x1b>(v, b1);   // lane ^ 3
-  v = Exchange<0xb1>(v, b0);
-  v = Exchange<0x141>(v, b2);  // lane ^ 7
-  v = Exchange<0x4e>(v, b1);   // lane ^ 2
-  v = Exchange<0xb1>(v, b0);
-  v = Exchange<0x140>(v, b3);  // lane ^ 15
-  const float up = Dpp<0x104, 0xf, 0x5>(v, v), o = Dpp<0x114, 0xf, 0xa>(up, v);  // lane ^ 4: + 4 or - 4
-  v = b2 ? Max(v, o) : Min(v, o);
-  v = Exchange<0x4e>(v, b1);
-  v = Exchange<0xb1>(v, b0);
-  return v;  // (lane l of the 16: the l-th largest)
-}
 // The k-th largest (k <= 16) of 16 lanes' pairs, in all lanes.
 __device__ inline float RowKthLargest(float a, float b, int k) {
-  const int l = threadIdx.x & 15;
   a = RowSort(a);
   b = RowSort(b);
-  // the 16 largest of both: a[l] against b[15 - l], a bitonic sequence that three more exchanges and
-  // the last sort
-  a = Max(a, Dpp<0x140>(b, b));
-  const float x = Dpp<kRowRor + 8>(a, a);  // lane ^ 8
-  a = !(l & 8) ? Max(a, x) : Min(a, x);
-  const float up = Dpp<0x104, 0xf, 0x5>(a, a), o = Dpp<0x114, 0xf, 0xa>(up, a);
-  a = !(l & 4) ? Max(a, o) : Min(a, o);
-  a = Exchange<0x4e>(a, !(l & 2));
-  a = Exchange<0xb1>(a, !(l & 1));
-  return __int_as_float(__builtin_amdgcn_ds_bpermute(((threadIdx.x & 48) + k - 1) * 4, __float_as_int(a)));
+  // the 16 largest of both are the larger of the l-th and the (15 - l)-th: a bitonic sequence
+  a = RowMerge(Max(a, Dpp<0x140>(b, b)));
+  return OfLane(a, (threadIdx.x & 48) + k - 1);
 }
 
 constexpr int kShortTop = 16;  // alternatives
@@ -885,13 +947,7 @@ __global__ __launch_bounds__(kBlock) void ScoresShortKernel(const ScoresArgs a) 
   const int n = a.r.vocab;
   U4 r[NCH];
   LoadUnit<T, NCH, 16>(x, n, l, r);
-  int64_t tok = -1;
-  float at_tok = 0.0f;
-  if (a.tokens) {
-    tok = IdAt(a.tokens, a.token64, row);
-    if (tok < 0 || tok >= n) tok = -1;
-    if (tok >= 0) at_tok = T::Load(x + tok);
-  }
+  const TokenLogit tok = LoadToken<T>(a, row, x);
   // the maxima of a lane's 16 bytes, and of the even and the odd ones of these
   float cm[NCH], half[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -924,11 +980,7 @@ __global__ __launch_bounds__(kBlock) void ScoresShortKernel(const ScoresArgs a) 
   s1 = fmaf(-exponent.delta, s0, s1) * less;
   s0 *= less;
   const float ls = LogSum(s0);
-  if (l == 0) {
-    if (a.tokens) a.logp[row] = tok >= 0 ? (at_tok - base) - ls : 0.0f;
-    a.entropy[row] = s0 == 0.0f ? 0.0f : ls - kLn2 * (s1 / s0);
-    *reinterpret_cast<float2 *>(a.stats + 2 * static_cast<size_t>(row)) = float2{m, s0};
-  }
+  if (l == 0) WriteRowScores(a, row, tok, m, s0, s1);
   if (!TOP) return;
 
   const int k = a.k;
@@ -1301,17 +1353,20 @@ __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a)
   const int tid = threadIdx.x;
   const Unit u = GetUnit(a.r, blockIdx.x * static_cast<uint32_t>(a.r.nseg));
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
+  const Partial *part = a.part + static_cast<size_t>(u.row) * a.r.nseg;
+  const Partial mine = FirstPartial(part, a.r.nseg);
   Slots<kBlock> t;
   t.any = false;
+  float xs[1];
   if (w != 0.0f) {
     LoadSlots<kBlock>(a, u.row, tid, t);
+    LoadAtSlots<T, kBlock>(RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u), t, xs);
     SoftmaxSlots<kBlock>(a, t, list, tid);
   }
   float m = 0.0f, s0 = 0.0f, loss = 0.0f;
   if (t.any) {
-    float s1, xs[1];
-    LoadAtSlots<T, kBlock>(RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u), t, xs);
-    JoinPartials(a.part + static_cast<size_t>(u.row) * a.r.nseg, a.r.nseg, a.k2, red, &m, &s0, &s1);
+    float s1;
+    JoinPartials(part, mine, a.r.nseg, a.k2, red, &m, &s0, &s1);
     loss = Divergence<kBlock>(a, t, xs, m, LogSum(s0), list.red[4]);
   }
   if (tid == 0) {
@@ -1404,7 +1459,7 @@ enum Purpose {
   kFused,   // loss and gradient
   kPieces,  // a gradient whose statistics are known: any part of a row by itself
 };
-Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what) {
+Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what, int top) {
   const int64_t bytes = vocab * ElemBytes(dtype), vec = 16 / ElemBytes(dtype);
   const int whole = static_cast<int>(vocab);
   if (bytes <= 2048) return {64, 2, whole, 1};
@@ -1415,7 +1470,8 @@ Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what) {
   if (what == kFused && bytes <= 262144 && rows >= 128) return {1024, 16, whole, 1};
   Plan p{kBlock, 8, 0, 0};
   int64_t cap = 32768;
-  while (cap > 4096 && rows * ((bytes + cap - 1) / cap) < 64) cap /= 2;
+  while (cap > 4096 && rows * ((bytes + cap - 1) / cap) < 64 && 2 * top * ((bytes + cap - 1) / cap) <= kHeld * kBlock)
+    cap /= 2;
   cap /= ElemBytes(dtype);
   p.nseg = static_cast<int>((vocab + cap - 1) / cap);
   // equal segments, whole vectors
@@ -1424,7 +1480,7 @@ Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what) {
   return p;
 }
 
-int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64_t *rows) {
+int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64_t *rows, int top = 0) {
   if (!r || r->batch < 0 || r->steps < 0) return SetError(KD_E_INVALID, "bad argument: rows");
   if (r->dtype != KD_DTYPE_F32 && r->dtype != KD_DTYPE_F16 && r->dtype != KD_DTYPE_BF16)
     return SetError(KD_E_INVALID, "bad argument: dtype of the logits");
@@ -1433,7 +1489,7 @@ int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64
   if (r->batch > INT32_MAX || r->steps > INT32_MAX || r->batch * r->steps > INT32_MAX)
     return SetError(KD_E_INVALID, "bad argument: more than 2^31 - 1 rows");
   *rows = r->batch * r->steps;
-  *plan = MakePlan(r->vocab, r->dtype, *rows, what);
+  *plan = MakePlan(r->vocab, r->dtype, *rows, what, top);
   // (a grid has fewer than 2^32 threads)
   if (*rows * plan->nseg > ((int64_t(1) << 32) - 1) / plan->tpu)
     return SetError(KD_E_INVALID, "bad argument: rows x vocab is too large for one call");
@@ -1549,7 +1605,7 @@ size_t kd_token_scores_workspace(const kd_frame_rows *rows, int32_t top) {
   Rows r;
   Plan p;
   int64_t n;
-  if (CheckRows(rows, kValues, &r, &p, &n) || top < 0 || top > kMaxTop || p.nseg == 1) return 0;
+  if (top < 0 || CheckRows(rows, kValues, &r, &p, &n, top) || top > kMaxTop || p.nseg == 1) return 0;
   const size_t units = static_cast<size_t>(n) * p.nseg;
   return Align(units * sizeof(Partial)) + units * top * sizeof(uint64_t);
 }
@@ -1561,7 +1617,7 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
     ScoresArgs a{};
     Plan p;
     int64_t n;
-    if (int rc = CheckRows(rows, kValues, &a.r, &p, &n)) return rc;
+    if (int rc = CheckRows(rows, kValues, &a.r, &p, &n, std::max(top, 0))) return rc;
     if (top < 0 || top > kMaxTop) return SetError(KD_E_INVALID, "bad argument: top must be between 0 and 64");
     if (tokens && token_bytes != 4 && token_bytes != 8)
       return SetError(KD_E_INVALID, "bad argument: token_bytes must be 4 or 8");
