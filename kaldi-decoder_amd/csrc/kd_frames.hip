@@ -123,16 +123,19 @@ template <int TPU>
 constexpr int kThreads = TPU < kBlock ? kBlock : TPU;  // of a workgroup
 template <int TPU>
 __device__ inline int UnitLane() {
-  return TPU == 64 ? (threadIdx.x & 63) : threadIdx.x;
+  return TPU < kBlock ? (threadIdx.x & (TPU - 1)) : threadIdx.x;
 }
-// Which of a workgroup's units a wave belongs to, and the unit's number.
+// Which of a workgroup's units a lane belongs to, and the unit's number.  A wave's (TPU 64) is the
+// same in all its lanes; 16 lanes (a DPP row) are the smallest unit.
 template <int TPU>
 __device__ inline int UnitInBlock() {
-  return TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  return TPU == 16 ? threadIdx.x >> 4 : TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
 }
 template <int TPU>
+constexpr int kUnits = kThreads<TPU> / TPU;  // in a workgroup
+template <int TPU>
 __device__ inline uint32_t UnitNumber() {
-  return TPU == 64 ? blockIdx.x * kWaves + UnitInBlock<TPU>() : blockIdx.x;
+  return blockIdx.x * kUnits<TPU> + UnitInBlock<TPU>();
 }
 
 // Lane `tid` of a unit holds 16 bytes of columns from (c * TPU + tid) * kVec on in r[c]: consecutive
@@ -244,7 +247,7 @@ __device__ inline float WaveSum(float v) {
   return Lane63(v + Dpp<0x143, 0xc>(0.0f, v));
 }
 
-// A unit of one wave (TPU 64) is never synchronised with the workgroup's others.
+// A unit of a wave or less is never synchronised with the workgroup's others.
 template <int TPU>
 __device__ inline void UnitSync() {
   if (TPU > 64) {
@@ -258,6 +261,7 @@ __device__ inline void UnitSync() {
 // `red`: one float a wave, not written again before the unit's next barrier but one.
 template <int TPU>
 __device__ inline float UnitMax(float v, float *red) {
+  if (TPU == 16) return RowMax(v);
   v = WaveMax(v);
   if (TPU == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -276,6 +280,7 @@ __device__ inline float SumOf(const float *red) {
 }
 template <int TPU>
 __device__ inline float UnitSum(float v, float *red) {
+  if (TPU == 16) return RowSum(v);
   v = WaveSum(v);
   if (TPU == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -710,11 +715,10 @@ __device__ inline void WriteNoTop(float *v, int32_t *i, float val, int k, int ti
 
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
 __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a) {
-  constexpr int kUnits = kThreads<TPU> / TPU;
-  __shared__ Scratch<TPU> scratch[TOP || TPU > 64 ? kUnits : 1];
+  __shared__ Scratch<TPU> scratch[TOP || TPU > 64 ? kUnits<TPU> : 1];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
-  if (TPU == 64 && unit >= a.r.rows) return;
+  if (TPU < kBlock && unit >= a.r.rows) return;
   Scratch<TPU> &s = scratch[TOP || TPU > 64 ? UnitInBlock<TPU>() : 0];
   const Unit u = GetUnit(a.r, unit);
   if (u.skip) {
@@ -935,8 +939,8 @@ template <class T, int NCH, bool TOP>
 __global__ __launch_bounds__(kBlock) void ScoresShortKernel(const ScoresArgs a) {
   __shared__ uint64_t lists[TOP ? kBlock / 16 : 1][TOP ? kShortCap : 1];
   __shared__ uint8_t chunk_lists[TOP ? kBlock / 16 : 1][TOP ? kShortCap : 1];
-  const int l = threadIdx.x & 15;
-  const uint32_t row = blockIdx.x * (kBlock / 16) + (threadIdx.x >> 4);
+  const int l = UnitLane<16>();
+  const uint32_t row = UnitNumber<16>();
   if (row >= a.r.rows) return;
   const Unit u = GetUnit(a.r, row);
   if (u.skip) {
@@ -1106,7 +1110,7 @@ template <class T, int NCH, int TPU>
 __global__ __launch_bounds__(kThreads<TPU>) void ScoresGradKernel(const ScoresGradArgs a) {
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
-  if (TPU == 64 && unit >= a.r.rows) return;
+  if (TPU < kBlock && unit >= a.r.rows) return;
   const Unit u = GetUnit(a.r, unit);
   typename T::Store *dx =
       const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)) + u.lo;
@@ -1164,26 +1168,28 @@ __device__ inline float TeacherValue(const DistillArgs &a, size_t at) {
 }
 
 // A unit's teacher: lane `tid` holds slots tid, tid + TPU, ...; all of them also in LDS.
-template <int TPU>
+// (SN slots a lane: 256 in a unit of a wave or more, 16 or 64 in one of 16 lanes.)
+template <int TPU, int SN>
+constexpr int kListed = TPU * SN < kMaxSlots ? TPU * SN : kMaxSlots;
+template <int TPU, int SN>
 struct TeacherList {
-  int id[kMaxSlots];
-  float q[kMaxSlots];
-  float red[5][TPU / 64];
+  int id[kListed<TPU, SN>];
+  float q[kListed<TPU, SN>];
+  float red[5][TPU < 64 ? 1 : TPU / 64];
 };
-template <int TPU>
+template <int TPU, int SN>
 struct Slots {
-  static constexpr int kN = TPU < kMaxSlots ? kMaxSlots / TPU : 1;
-  int id[kN];   // -1: empty
-  float u[kN];  // (logit - largest) / temperature
-  float q[kN];
+  int id[SN];   // -1: empty
+  float u[SN];  // (logit - largest) / temperature
+  float q[SN];
   float log_usum;
   bool any;
 };
 
-template <int TPU>
-__device__ inline void LoadSlots(const DistillArgs &a, uint32_t row, int tid, Slots<TPU> &t) {
+template <int TPU, int SN>
+__device__ inline void LoadSlots(const DistillArgs &a, uint32_t row, int tid, Slots<TPU, SN> &t) {
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) {
+  for (int i = 0; i < SN; ++i) {
     t.id[i] = -1;
     t.u[i] = -INFINITY;
     const int k = i * TPU + tid;
@@ -1198,19 +1204,19 @@ __device__ inline void LoadSlots(const DistillArgs &a, uint32_t row, int tid, Sl
   }
 }
 // q = softmax(u / temperature) over the filled slots.
-template <int TPU>
-__device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, TeacherList<TPU> &list, int tid) {
+template <int TPU, int SN>
+__device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU, SN> &t, TeacherList<TPU, SN> &list, int tid) {
   float um = -INFINITY, sum = 0.0f;
   bool nan = false;
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) {
+  for (int i = 0; i < SN; ++i) {
     um = fmaxf(um, t.u[i]);
     nan |= isnan(t.u[i]);
   }
   um = UnitMax<TPU>(nan ? INFINITY : um, list.red[0]);  // (inf - inf below: NaN for the whole row)
   t.any = um != -INFINITY;
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) {
+  for (int i = 0; i < SN; ++i) {
     t.u[i] = (t.u[i] - Base(um)) * a.inv_t;
     t.q[i] = um == INFINITY && t.id[i] >= 0 ? NAN : expf(t.u[i]);
     sum += t.q[i];
@@ -1218,7 +1224,7 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, Teacher
   sum = UnitSum<TPU>(sum, list.red[1]);
   t.log_usum = logf(sum);
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) {
+  for (int i = 0; i < SN; ++i) {
     t.q[i] = t.q[i] / sum;
     const int k = i * TPU + tid;
     if (k < a.slots) {
@@ -1230,12 +1236,12 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU> &t, Teacher
 }
 
 // sum_k q_k (log q_k - log p_k), log p_k = (x_k - m) / temperature - ls; xs: the students' logits at the slots.
-template <int TPU>
-__device__ inline float Divergence(const DistillArgs &a, const Slots<TPU> &t, const float (&xs)[Slots<TPU>::kN],
+template <int TPU, int SN>
+__device__ inline float Divergence(const DistillArgs &a, const Slots<TPU, SN> &t, const float (&xs)[SN],
                                    float m, float ls, float *red) {
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) {
+  for (int i = 0; i < SN; ++i) {
     // (the logit's product is formed with q / temperature: (lowest - m) / temperature alone may overflow)
     const float d = xs[i] - Base(m), each = (t.u[i] - t.log_usum) + ls;
     if (t.id[i] >= 0 && t.q[i] != 0.0f) sum += fmaf(t.q[i], each, -(t.q[i] * a.inv_t) * d);
@@ -1246,9 +1252,9 @@ __device__ inline float Divergence(const DistillArgs &a, const Slots<TPU> &t, co
 // Writes a unit's gradient: coef (p_j - sum of the q of the slots that name column j).  The slots'
 // columns are written again behind the others, by one lane each (slots that name one column write
 // the same value).
-template <class T, int NCH, int TPU>
-__device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, const U4 (&r)[NCH], const Slots<TPU> &t,
-                                        const float (&xs)[Slots<TPU>::kN], const TeacherList<TPU> &list, float m,
+template <class T, int NCH, int TPU, int SN>
+__device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, const U4 (&r)[NCH], const Slots<TPU, SN> &t,
+                                        const float (&xs)[SN], const TeacherList<TPU, SN> &list, float m,
                                         float s0, float coef, int tid) {
   typename T::Store *dx =
       const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)) + u.lo;
@@ -1261,7 +1267,7 @@ __device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, con
   });
   UnitSync<TPU>();
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) {
+  for (int i = 0; i < SN; ++i) {
     if (i * TPU >= a.slots) break;
     const int at = t.id[i] - u.lo;
     const bool mine = t.id[i] >= 0 && at >= 0 && at < u.n;
@@ -1274,32 +1280,32 @@ __device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, con
 }
 
 // The students' logits at a lane's slots.
-template <class T, int TPU>
-__device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU> &t, float (&xs)[Slots<TPU>::kN]) {
+template <class T, int TPU, int SN>
+__device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU, SN> &t, float (&xs)[SN]) {
 #pragma unroll
-  for (int i = 0; i < Slots<TPU>::kN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
+  for (int i = 0; i < SN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
 }
 
 // Whole rows: loss, and with GRAD the gradient from the registers that the statistics were taken of.
-template <class T, int NCH, int TPU, bool GRAD>
+template <class T, int NCH, int TPU, int SN, bool GRAD>
 __global__ __launch_bounds__(kThreads<TPU>) void DistillKernel(const DistillArgs a) {
-  __shared__ TeacherList<TPU> lists[kThreads<TPU> / TPU];
+  __shared__ TeacherList<TPU, SN> lists[kUnits<TPU>];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
-  if (TPU == 64 && unit >= a.r.rows) return;
+  if (TPU < kBlock && unit >= a.r.rows) return;
   const Unit u = GetUnit(a.r, unit);
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
-  TeacherList<TPU> &list = lists[UnitInBlock<TPU>()];
-  Slots<TPU> t;
+  TeacherList<TPU, SN> &list = lists[UnitInBlock<TPU>()];
+  Slots<TPU, SN> t;
   t.any = false;
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
   U4 r[NCH];
-  float xs[Slots<TPU>::kN];
+  float xs[SN];
   if (w != 0.0f) {
-    LoadSlots<TPU>(a, u.row, tid, t);
+    LoadSlots<TPU, SN>(a, u.row, tid, t);
     LoadUnit<T, NCH, TPU>(x, u.n, tid, r);
-    LoadAtSlots<T, TPU>(x, t, xs);
-    SoftmaxSlots<TPU>(a, t, list, tid);
+    LoadAtSlots<T, TPU, SN>(x, t, xs);
+    SoftmaxSlots<TPU, SN>(a, t, list, tid);
   }
   if (!t.any) {  // (the same in all lanes of the unit)
     if (tid == 0) {
@@ -1330,7 +1336,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void DistillKernel(const DistillArgs
   }
   s0 = UnitSum<TPU>(s0, list.red[3]) * __builtin_amdgcn_exp2f(-exponent.delta);
   const float ls = LogSum(s0);
-  const float loss = Divergence<TPU>(a, t, xs, m, ls, list.red[4]);
+  const float loss = Divergence<TPU, SN>(a, t, xs, m, ls, list.red[4]);
   if (tid == 0) {
     if (a.loss) a.loss[u.row] = w * loss;
     if (a.stats) {
@@ -1341,33 +1347,33 @@ __global__ __launch_bounds__(kThreads<TPU>) void DistillKernel(const DistillArgs
   if (GRAD) {
     NewPass(r);
     const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
-    WriteDistillGrad<T, NCH, TPU>(a, u, r, t, xs, list, m, s0, coef, tid);
+    WriteDistillGrad<T, NCH, TPU, SN>(a, u, r, t, xs, list, m, s0, coef, tid);
   }
 }
 
 // Split rows: the statistics of a row from its segments', and its loss.
 template <class T>
 __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a) {
-  __shared__ TeacherList<kBlock> list;
+  __shared__ TeacherList<kBlock, 1> list;
   __shared__ float red[3][kWaves];
   const int tid = threadIdx.x;
   const Unit u = GetUnit(a.r, blockIdx.x * static_cast<uint32_t>(a.r.nseg));
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
   const Partial *part = a.part + static_cast<size_t>(u.row) * a.r.nseg;
   const Partial mine = FirstPartial(part, a.r.nseg);
-  Slots<kBlock> t;
+  Slots<kBlock, 1> t;
   t.any = false;
   float xs[1];
   if (w != 0.0f) {
-    LoadSlots<kBlock>(a, u.row, tid, t);
-    LoadAtSlots<T, kBlock>(RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u), t, xs);
-    SoftmaxSlots<kBlock>(a, t, list, tid);
+    LoadSlots<kBlock, 1>(a, u.row, tid, t);
+    LoadAtSlots<T, kBlock, 1>(RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u), t, xs);
+    SoftmaxSlots<kBlock, 1>(a, t, list, tid);
   }
   float m = 0.0f, s0 = 0.0f, loss = 0.0f;
   if (t.any) {
     float s1;
     JoinPartials(part, mine, a.r.nseg, a.k2, red, &m, &s0, &s1);
-    loss = Divergence<kBlock>(a, t, xs, m, LogSum(s0), list.red[4]);
+    loss = Divergence<kBlock, 1>(a, t, xs, m, LogSum(s0), list.red[4]);
   }
   if (tid == 0) {
     if (a.loss) a.loss[u.row] = t.any ? w * loss : 0.0f;
@@ -1377,27 +1383,27 @@ __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a)
 }
 
 // The gradient of rows or segments whose statistics are known.
-template <class T, int NCH, int TPU>
+template <class T, int NCH, int TPU, int SN>
 __global__ __launch_bounds__(kThreads<TPU>) void DistillGradKernel(const DistillArgs a) {
-  __shared__ TeacherList<TPU> lists[kThreads<TPU> / TPU];
+  __shared__ TeacherList<TPU, SN> lists[kUnits<TPU>];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
-  if (TPU == 64 && unit >= a.r.rows) return;
+  if (TPU < kBlock && unit >= a.r.rows) return;
   const Unit u = GetUnit(a.r, unit);
   const float w = u.skip ? 0.0f : a.weights ? a.weights[u.row] : 1.0f;
-  TeacherList<TPU> &list = lists[UnitInBlock<TPU>()];
-  Slots<TPU> t;
+  TeacherList<TPU, SN> &list = lists[UnitInBlock<TPU>()];
+  Slots<TPU, SN> t;
   t.any = false;
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
   U4 r[NCH];
-  float xs[Slots<TPU>::kN];
+  float xs[SN];
   if (w != 0.0f) {
-    LoadSlots<TPU>(a, u.row, tid, t);
+    LoadSlots<TPU, SN>(a, u.row, tid, t);
     LoadUnit<T, NCH, TPU>(x + u.lo, u.n, tid, r);
-    LoadAtSlots<T, TPU>(x, t, xs);
+    LoadAtSlots<T, TPU, SN>(x, t, xs);
     // (its barriers stand between every lane's loads of the slots' logits and the first stores: the
     // gradient may be written over the logits)
-    SoftmaxSlots<TPU>(a, t, list, tid);
+    SoftmaxSlots<TPU, SN>(a, t, list, tid);
   }
   if (!t.any) {
     StoreZeros<T, NCH, TPU>(
@@ -1406,7 +1412,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void DistillGradKernel(const Distill
   }
   const float m = a.stats[2 * static_cast<size_t>(u.row)], s0 = a.stats[2 * static_cast<size_t>(u.row) + 1];
   const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
-  WriteDistillGrad<T, NCH, TPU>(a, u, r, t, xs, list, m, s0, coef, tid);
+  WriteDistillGrad<T, NCH, TPU, SN>(a, u, r, t, xs, list, m, s0, coef, tid);
 }
 
 // ---- host side -----------------------------------------------------------------------------------
@@ -1459,9 +1465,11 @@ enum Purpose {
   kFused,   // loss and gradient
   kPieces,  // a gradient whose statistics are known: any part of a row by itself
 };
-Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what, int top) {
+Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what, int top, bool narrow) {
   const int64_t bytes = vocab * ElemBytes(dtype), vec = 16 / ElemBytes(dtype);
   const int whole = static_cast<int>(vocab);
+  // Short rows, four to a wave (the lists of a longer teacher take a wave's lanes: `narrow`).
+  if (bytes <= 2048 && narrow) return {16, bytes <= 512 ? 2 : 8, whole, 1};
   if (bytes <= 2048) return {64, 2, whole, 1};
   if (bytes <= 8192) return {64, 8, whole, 1};
   if (bytes <= 32768) return {kBlock, 8, whole, 1};
@@ -1480,7 +1488,7 @@ Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what, int top) {
   return p;
 }
 
-int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64_t *rows, int top = 0) {
+int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64_t *rows, int top, bool narrow) {
   if (!r || r->batch < 0 || r->steps < 0) return SetError(KD_E_INVALID, "bad argument: rows");
   if (r->dtype != KD_DTYPE_F32 && r->dtype != KD_DTYPE_F16 && r->dtype != KD_DTYPE_BF16)
     return SetError(KD_E_INVALID, "bad argument: dtype of the logits");
@@ -1489,7 +1497,7 @@ int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64
   if (r->batch > INT32_MAX || r->steps > INT32_MAX || r->batch * r->steps > INT32_MAX)
     return SetError(KD_E_INVALID, "bad argument: more than 2^31 - 1 rows");
   *rows = r->batch * r->steps;
-  *plan = MakePlan(r->vocab, r->dtype, *rows, what, top);
+  *plan = MakePlan(r->vocab, r->dtype, *rows, what, top, narrow);
   // (a grid has fewer than 2^32 threads)
   if (*rows * plan->nseg > ((int64_t(1) << 32) - 1) / plan->tpu)
     return SetError(KD_E_INVALID, "bad argument: rows x vocab is too large for one call");
@@ -1533,8 +1541,8 @@ int CheckGrad(const kd_frame_rows *r, void *dx, int64_t batch_stride, int64_t ro
 }
 
 uint32_t Blocks(const Rows &r, const Plan &p) {
-  const uint64_t units = static_cast<uint64_t>(r.rows) * r.nseg;
-  return static_cast<uint32_t>(p.tpu == 64 ? (units + kWaves - 1) / kWaves : units);
+  const uint64_t units = static_cast<uint64_t>(r.rows) * r.nseg, per = std::max(kBlock / p.tpu, 1);
+  return static_cast<uint32_t>((units + per - 1) / per);
 }
 
 // f(T{}, NCH, TPU as constants) for a plan.
@@ -1542,14 +1550,27 @@ template <int N>
 struct Int {
   static constexpr int value = N;
 };
-template <Purpose WHAT, class T, class F>
+// Which units of short rows a kernel is made for.
+enum ShortUnits { kNone, kBySixteen, kByWave, kByBoth };
+template <Purpose WHAT, ShortUnits SHORT, class T, class F>
 int ForPlan(const Plan &p, F f) {
-  if (p.tpu == 64) return p.nch == 2 ? f(T{}, Int<2>{}, Int<64>{}) : f(T{}, Int<8>{}, Int<64>{});
+  if constexpr (SHORT == kBySixteen || SHORT == kByBoth)
+    if (p.tpu == 16) return p.nch == 2 ? f(T{}, Int<2>{}, Int<16>{}) : f(T{}, Int<8>{}, Int<16>{});
+  if constexpr (SHORT == kByWave || SHORT == kByBoth)
+    if (p.tpu == 64 && p.nch == 2) return f(T{}, Int<2>{}, Int<64>{});
+  if (p.tpu == 64) return f(T{}, Int<8>{}, Int<64>{});
   if constexpr (WHAT != kPieces)
     if (p.tpu == 512) return f(T{}, Int<8>{}, Int<512>{});
   if constexpr (WHAT == kFused)
     if (p.tpu == 1024) return p.nch == 8 ? f(T{}, Int<8>{}, Int<1024>{}) : f(T{}, Int<16>{}, Int<1024>{});
   return f(T{}, Int<8>{}, Int<kBlock>{});
+}
+// f(SN as a constant): slots a lane.
+constexpr int kShortSlots = 64;  // of a teacher of short rows
+template <int TPU, class F>
+int ForSlots(int slots, F f) {
+  if constexpr (TPU == 16) return slots <= 16 ? f(Int<1>{}) : f(Int<4>{});
+  else return f(Int<(TPU < kMaxSlots ? kMaxSlots / TPU : 1)>{});
 }
 template <class F>
 int ForType(int dtype, F f) {
@@ -1575,7 +1596,9 @@ int LaunchScores(const kd_frame_rows *rows, const ScoresArgs &a, const Plan &pla
     if constexpr (SPLIT) {
       return Launch(ScoresKernel<T, 8, kBlock, true, ENT, TOP>, Blocks(a.r, plan), a, stream);
     } else {
-      return ForPlan<kValues, T>(plan, [&](auto tt, auto nch, auto tpu) {
+      // (short rows of few alternatives are LaunchShort's: without alternatives no wave takes one)
+      constexpr ShortUnits kShort = TOP ? kByWave : kNone;
+      return ForPlan<kValues, kShort, T>(plan, [&](auto tt, auto nch, auto tpu) {
         return Launch(ScoresKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value, false, ENT, TOP>,
                       Blocks(a.r, plan), a, stream, kThreads<decltype(tpu)::value>);
       });
@@ -1583,17 +1606,12 @@ int LaunchScores(const kd_frame_rows *rows, const ScoresArgs &a, const Plan &pla
   });
 }
 
-bool IsShort(int64_t vocab, int dtype) { return vocab * ElemBytes(dtype) <= 16 * 16 * 8; }
 template <bool TOP>
-int LaunchShort(const kd_frame_rows *rows, const ScoresArgs &a, void *stream) {
-  const uint32_t blocks = (a.r.rows + kBlock / 16 - 1) / (kBlock / 16);
-  const int64_t bytes = rows->vocab * ElemBytes(rows->dtype);
+int LaunchShort(const kd_frame_rows *rows, const ScoresArgs &a, const Plan &plan, void *stream) {
   return ForType(rows->dtype, [&](auto t) {
     using T = decltype(t);
-    return bytes <= 256    ? Launch(ScoresShortKernel<T, 1, TOP>, blocks, a, stream)
-           : bytes <= 512  ? Launch(ScoresShortKernel<T, 2, TOP>, blocks, a, stream)
-           : bytes <= 1024 ? Launch(ScoresShortKernel<T, 4, TOP>, blocks, a, stream)
-                           : Launch(ScoresShortKernel<T, 8, TOP>, blocks, a, stream);
+    return plan.nch == 2 ? Launch(ScoresShortKernel<T, 2, TOP>, Blocks(a.r, plan), a, stream)
+                         : Launch(ScoresShortKernel<T, 8, TOP>, Blocks(a.r, plan), a, stream);
   });
 }
 
@@ -1605,7 +1623,7 @@ size_t kd_token_scores_workspace(const kd_frame_rows *rows, int32_t top) {
   Rows r;
   Plan p;
   int64_t n;
-  if (top < 0 || CheckRows(rows, kValues, &r, &p, &n, top) || top > kMaxTop || p.nseg == 1) return 0;
+  if (top < 0 || CheckRows(rows, kValues, &r, &p, &n, top, top <= kShortTop) || top > kMaxTop || p.nseg == 1) return 0;
   const size_t units = static_cast<size_t>(n) * p.nseg;
   return Align(units * sizeof(Partial)) + units * top * sizeof(uint64_t);
 }
@@ -1617,7 +1635,7 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
     ScoresArgs a{};
     Plan p;
     int64_t n;
-    if (int rc = CheckRows(rows, kValues, &a.r, &p, &n, std::max(top, 0))) return rc;
+    if (int rc = CheckRows(rows, kValues, &a.r, &p, &n, std::max(top, 0), top <= kShortTop)) return rc;
     if (top < 0 || top > kMaxTop) return SetError(KD_E_INVALID, "bad argument: top must be between 0 and 64");
     if (tokens && token_bytes != 4 && token_bytes != 8)
       return SetError(KD_E_INVALID, "bad argument: token_bytes must be 4 or 8");
@@ -1638,9 +1656,7 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
     a.top_i = top_ids;
     DeviceGuard guard(rows->device);
     if (guard.error() != hipSuccess) return HipFail("hipSetDevice", guard.error());
-    // Short rows, four to a wave; more than 16 alternatives need the 64 groups of a whole wave.
-    if (IsShort(a.r.vocab, rows->dtype) && top <= kShortTop)
-      return top ? LaunchShort<true>(rows, a, stream) : LaunchShort<false>(rows, a, stream);
+    if (p.tpu == 16) return top ? LaunchShort<true>(rows, a, p, stream) : LaunchShort<false>(rows, a, p, stream);
     if (p.nseg == 1)
       return top ? LaunchScores<false, true, true>(rows, a, p, stream)
                  : LaunchScores<false, true, false>(rows, a, p, stream);
@@ -1666,7 +1682,7 @@ int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t 
     ScoresGradArgs a{};
     Plan p;
     int64_t n;
-    if (int rc = CheckRows(rows, kPieces, &a.r, &p, &n)) return rc;
+    if (int rc = CheckRows(rows, kPieces, &a.r, &p, &n, 0, true)) return rc;
     if (tokens && token_bytes != 4 && token_bytes != 8)
       return SetError(KD_E_INVALID, "bad argument: token_bytes must be 4 or 8");
     if (!n) return KD_OK;
@@ -1681,7 +1697,7 @@ int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t 
     DeviceGuard guard(rows->device);
     if (guard.error() != hipSuccess) return HipFail("hipSetDevice", guard.error());
     return ForType(rows->dtype, [&](auto t) {
-      return ForPlan<kPieces, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+      return ForPlan<kPieces, kBySixteen, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
         return Launch(ScoresGradKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value>, Blocks(a.r, p), a,
                       stream, kThreads<decltype(tpu)::value>);
       });
@@ -1693,7 +1709,7 @@ size_t kd_distill_loss_workspace(const kd_frame_rows *rows, int32_t with_grad) {
   Rows r;
   Plan p;
   int64_t n;
-  if (CheckRows(rows, with_grad ? kFused : kValues, &r, &p, &n) || p.nseg == 1) return 0;
+  if (CheckRows(rows, with_grad ? kFused : kValues, &r, &p, &n, 0, false) || p.nseg == 1) return 0;
   return Align(static_cast<size_t>(n) * p.nseg * sizeof(Partial)) + Align(static_cast<size_t>(n) * 8);
 }
 
@@ -1706,7 +1722,7 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
     int64_t n;
     // stats given and no loss asked for: the statistics of an earlier call, the gradient alone
     const bool known = !loss && stats;
-    if (int rc = CheckRows(rows, known ? kPieces : grad ? kFused : kValues, &a.r, &p, &n)) return rc;
+    if (int rc = CheckRows(rows, known ? kPieces : grad ? kFused : kValues, &a.r, &p, &n, 0, teacher && teacher->slots <= kShortSlots)) return rc;
     if (!teacher || teacher->slots < 1 || teacher->slots > kMaxSlots)
       return SetError(KD_E_INVALID, "bad argument: a teacher lists between 1 and 256 tokens a row");
     if (teacher->id_bytes != 4 && teacher->id_bytes != 8)
@@ -1755,25 +1771,27 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
     }
     if (p.nseg > 1 || known) {
       return ForType(rows->dtype, [&](auto t) {
-        return ForPlan<kPieces, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
-          return Launch(DistillGradKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value>, Blocks(a.r, p), a,
-                        stream);
+        return ForPlan<kPieces, kByBoth, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+          return ForSlots<decltype(tpu)::value>(a.slots, [&](auto sn) {
+            return Launch(DistillGradKernel<decltype(tt), decltype(nch)::value, decltype(tpu)::value, decltype(sn)::value>,
+                          Blocks(a.r, p), a, stream);
+          });
         });
       });
     }
-    return ForType(rows->dtype, [&](auto t) {
-      if (grad)
-        return ForPlan<kFused, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
+    auto whole = [&](auto what, auto with_grad) {
+      return ForType(rows->dtype, [&](auto t) {
+        return ForPlan<static_cast<Purpose>(decltype(what)::value), kByBoth, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
           constexpr int TPU = decltype(tpu)::value;
-          return Launch(DistillKernel<decltype(tt), decltype(nch)::value, TPU, true>, Blocks(a.r, p), a, stream,
-                        kThreads<TPU>);
+          return ForSlots<TPU>(a.slots, [&](auto sn) {
+            return Launch(DistillKernel<decltype(tt), decltype(nch)::value, TPU, decltype(sn)::value,
+                                        decltype(with_grad)::value != 0>,
+                          Blocks(a.r, p), a, stream, kThreads<TPU>);
+          });
         });
-      return ForPlan<kValues, decltype(t)>(p, [&](auto tt, auto nch, auto tpu) {
-        constexpr int TPU = decltype(tpu)::value;
-        return Launch(DistillKernel<decltype(tt), decltype(nch)::value, TPU, false>, Blocks(a.r, p), a, stream,
-                      kThreads<TPU>);
       });
-    });
+    };
+    return grad ? whole(Int<kFused>{}, Int<1>{}) : whole(Int<kValues>{}, Int<0>{});
   });
 }
 
