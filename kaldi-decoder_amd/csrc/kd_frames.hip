@@ -121,6 +121,12 @@ __device__ inline const typename T::Store *RowPtr(const void *x, int64_t batch_s
 
 template <int TPU>
 constexpr int kThreads = TPU < kBlock ? kBlock : TPU;  // of a workgroup
+// Waves a SIMD that a kernel is compiled for (1: as many as its registers allow).  Units of 512 lanes
+// take two a SIMD, so 68 registers instead of 64 would cost one unit in four (40.4 instead of 43.2 us
+// for 2048 rows of 32768 bf16 with 64 alternatives); the others lose a wave slot in eight at most, and
+// more by spilling.
+template <int TPU, int NCH>
+constexpr int kOccupancy = TPU == 512 || (TPU == 1024 && NCH <= 8) ? 8 : 1;
 template <int TPU>
 __device__ inline int UnitLane() {
   return TPU < kBlock ? (threadIdx.x & (TPU - 1)) : threadIdx.x;
@@ -341,6 +347,8 @@ struct Scratch {
   float group_max[kW == 1 ? 1 : 64 * kW];
   int place[kW == 1 ? 1 : kMaxRanked];
   uint64_t cand[kW][kList];  // Key
+  U4 raw[kW][kList / 2];     // 16 bytes with a candidate among them, and whose they were
+  uint16_t raw_of[kW][kList / 2];
 };
 
 // A whole number that orders as the value does (-0 and +0 alike).
@@ -430,27 +438,12 @@ __device__ inline float GroupThreshold(const float (&g)[2], Scratch<TPU> &s, int
   return s.threshold;
 }
 
-// What a selection reads, as f(value, column) with all lanes of a wave in step: a unit's registers
-// (`cm`: a lane's maximum of each; what none of the wave's lanes has an element of is passed over),
-template <class T, int NCH, int TPU>
-struct RegSource {
-  const U4 (&r)[NCH];
-  const float (&cm)[NCH];
-  int lo, n, tid;
-  template <class F>
-  __device__ void Each(float floor_v, F f) const {
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      if (__ballot(cm[c] >= floor_v)) {
-        const int first = lo + FirstCol<T>((c * TPU + tid) * T::kVec, n);
-#pragma unroll
-        for (int j = 0; j < T::kVec; ++j) f(T::Get(r[c], j), first + j);
-      }
-    }
-  }
-};
-// the same unit from memory (for the bisection, which is rare: over the registers it would make
-// every kernel hold its code many times over),
+// What a selection reads, as f(value, column) with all lanes of a wave in step: a list in memory (the
+// alternatives of a row's segments), in registers, or a unit's elements.  A unit in registers is
+// collected in two steps (CollectUnit).
+//
+// A unit from memory, for the bisection, which is rare: over the registers it would make every
+// kernel hold its code many times over.
 template <class T, int TPU>
 struct MemSource {
   static constexpr int kLowBit = sizeof(typename T::Store) == 4 ? 0 : 13;  // an f16's or bf16's lower bits are 0
@@ -464,7 +457,7 @@ struct MemSource {
     }
   }
 };
-// or the sorted lists of a row's segments, in memory (the first of all, then the second of all, ...:
+// The sorted lists of a row's segments, in memory (the first of all, then the second of all, ...:
 // a thread's share, whose maximum is one of the threshold's groups, has few of any one list's head).
 struct ListSource {
   static constexpr int kLowBit = 0;
@@ -530,6 +523,50 @@ __device__ inline void Collect(const SRC &src, Scratch<TPU> &s, float floor_v, P
   if (lane == 0) s.count[w] = n;
 }
 
+// The same of a unit's registers, in two steps: the 16 bytes that have such an element (`cm`: a lane's
+// maximum of each) are put into LDS, then a lane takes each and lists its elements -- a third of the
+// instructions, and an eighth of the code, of looking at each register's elements in turn.
+template <class T, int NCH, int TPU>
+__device__ inline void CollectUnit(const U4 (&r)[NCH], const float (&cm)[NCH], int lo, int cols, Scratch<TPU> &s,
+                                   float floor_v) {
+  constexpr int kList = Scratch<TPU>::kList;
+  const int lane = threadIdx.x & 63, w = TPU == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  int held = 0;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const bool mine = cm[c] >= floor_v;
+    const uint64_t m = __ballot(mine);
+    if (m) {
+      const int pos = held + Popc(m & below);
+      if (mine && pos < kList / 2) {
+        s.raw[w][pos] = r[c];
+        s.raw_of[w][pos] = static_cast<uint16_t>(c * TPU + UnitLane<TPU>());
+      }
+      held += Popc(m);
+    }
+  }
+  int n = held > kList / 2 ? kList + 1 : 0;  // (too many to hold: as too many candidates)
+  if (!n) {
+    UnitSync<64>();
+    for (int base = 0; base < held; base += 64) {
+      const bool have = base + lane < held;
+      const U4 v = s.raw[w][have ? base + lane : 0];
+      const int e = s.raw_of[w][have ? base + lane : 0] * T::kVec, first = FirstCol<T>(e, cols);
+#pragma unroll
+      for (int j = 0; j < T::kVec; ++j) {
+        const float x = T::Get(v, j);
+        const bool mine = have && first + j >= e && x >= floor_v;
+        const uint64_t m = __ballot(mine);
+        const int pos = n + Popc(m & below);
+        if (mine && pos < kList) s.cand[w][pos] = Key(x, lo + first + j);
+        n += Popc(m);
+      }
+    }
+  }
+  if (lane == 0) s.count[w] = n;
+}
+
 // The key of the k-th element itself, among those that reach `floor_v`; at least k do.
 template <int TPU, class SRC>
 __device__ __noinline__ uint64_t KthElement(const SRC src, int *red, float floor_v, int k) {
@@ -557,13 +594,13 @@ __device__ __noinline__ uint64_t KthElement(const SRC src, int *red, float floor
 
 // Puts the unit's K largest elements in order and hands (place, key) to `out`, once per place from
 // some lane; places without an element get key 0.  `threshold`: at least k of the unit's elements
-// reach it, or it is -inf or NaN.
-template <int TPU, class SRC, class MEM, class OUT>
-__device__ inline void SelectTop(const SRC &src, const MEM &mem, Scratch<TPU> &s, float threshold, int k, OUT out) {
+// reach it, or it is -inf or NaN.  `collect`: Collect or CollectUnit of the elements that reach a value.
+template <int TPU, class COLLECT, class MEM, class OUT>
+__device__ inline void SelectTop(COLLECT collect, const MEM &mem, Scratch<TPU> &s, float threshold, int k, OUT out) {
   constexpr int kW = TPU / 64, kList = Scratch<TPU>::kList;
   const int tid = UnitLane<TPU>();
   const float floor_v = fmaxf(threshold, kLowest);  // (-inf is no alternative)
-  Collect<TPU>(src, s, floor_v, [=](float v, int) { return v >= floor_v; });
+  collect(floor_v);
   if (TPU > 64)
     for (int a = tid; a < kMaxRanked; a += TPU) s.place[a] = 0;
   UnitSync<TPU>();
@@ -714,7 +751,7 @@ __device__ inline void WriteNoTop(float *v, int32_t *i, float val, int k, int ti
 }
 
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
-__global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a) {
+__global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresKernel(const ScoresArgs a) {
   __shared__ Scratch<TPU> scratch[TOP || TPU > 64 ? kUnits<TPU> : 1];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
@@ -780,7 +817,7 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
 
   if (SPLIT) {
     if (tid == 0) a.part[unit] = Partial{m, s0, s1, 0.0f};
-  } else if (tid == 0) {
+  } else if (tid == TPU - 1) {  // (not the wave that the threshold is up to)
     WriteRowScores(a, u.row, tok, m, s0, s1);
   }
   if (TOP) {
@@ -791,13 +828,13 @@ __global__ __launch_bounds__(kThreads<TPU>) void ScoresKernel(const ScoresArgs a
     }
     NewPass(r);
     const float threshold = GroupThreshold<TPU>(g, s, a.k);
-    const RegSource<T, NCH, TPU> src{r, cm, u.lo, u.n, tid};
+    auto collect = [&](float floor_v) { CollectUnit<T, NCH, TPU>(r, cm, u.lo, u.n, s, floor_v); };
     const MemSource<T, TPU> mem{x + u.lo, u.lo, u.n, tid};
     if (SPLIT) {
       uint64_t *list = a.part_top + at;
-      SelectTop<TPU>(src, mem, s, threshold, a.k, [=](int place, uint64_t key) { list[place] = key; });
+      SelectTop<TPU>(collect, mem, s, threshold, a.k, [=](int place, uint64_t key) { list[place] = key; });
     } else {
-      SelectTop<TPU>(src, mem, s, threshold, a.k, TopWriter{a.top_v + at, a.top_i + at, base, LogSum(s0)});
+      SelectTop<TPU>(collect, mem, s, threshold, a.k, TopWriter{a.top_v + at, a.top_i + at, base, LogSum(s0)});
     }
   }
 }
@@ -879,11 +916,16 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
     const float none[2] = {};
     const float threshold = GroupThreshold<kBlock>(none, s, k);
     const TopWriter out{tv, ti, Base(m), LogSum(s0)};
-    if (hold) {
-      SelectTop<kBlock>(held, list, s, threshold, k, out);
-    } else {
-      SelectTop<kBlock>(list, list, s, threshold, k, out);
-    }
+    SelectTop<kBlock>(
+        [&](float floor_v) {
+          auto reaches = [=](float v, int) { return v >= floor_v; };
+          if (hold) {
+            Collect<kBlock>(held, s, floor_v, reaches);
+          } else {
+            Collect<kBlock>(list, s, floor_v, reaches);
+          }
+        },
+        list, s, threshold, k, out);
   }
 }
 
@@ -1107,7 +1149,7 @@ struct ScoresGradArgs {
 // log s (t_j the exponent) that is e_j (A + B t_j) + g_logp [j = token]: A = (-g_logp - g_H (H - log s)) / s,
 // B = -ln 2 g_H / s.
 template <class T, int NCH, int TPU>
-__global__ __launch_bounds__(kThreads<TPU>) void ScoresGradKernel(const ScoresGradArgs a) {
+__global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresGradKernel(const ScoresGradArgs a) {
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
   if (TPU < kBlock && unit >= a.r.rows) return;
@@ -1288,7 +1330,7 @@ __device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU, 
 
 // Whole rows: loss, and with GRAD the gradient from the registers that the statistics were taken of.
 template <class T, int NCH, int TPU, int SN, bool GRAD>
-__global__ __launch_bounds__(kThreads<TPU>) void DistillKernel(const DistillArgs a) {
+__global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void DistillKernel(const DistillArgs a) {
   __shared__ TeacherList<TPU, SN> lists[kUnits<TPU>];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
@@ -1384,7 +1426,7 @@ __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a)
 
 // The gradient of rows or segments whose statistics are known.
 template <class T, int NCH, int TPU, int SN>
-__global__ __launch_bounds__(kThreads<TPU>) void DistillGradKernel(const DistillArgs a) {
+__global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void DistillGradKernel(const DistillArgs a) {
   __shared__ TeacherList<TPU, SN> lists[kUnits<TPU>];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();

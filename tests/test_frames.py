@@ -24,7 +24,7 @@ def _refused(rc, text):
     (dict(dtype=3), "dtype"), (dict(vocab=0), "vocab"), (dict(vocab=2**24 + 1), "vocab"), (dict(batch=-1), "rows"),
     (dict(steps=2**31), "2^31"), (dict(batch=2**20, steps=2**20), "2^31"), (dict(row_stride=-1), "stride"),
     (dict(logits=None), "logits"), (dict(logits=4098), "aligned"), (dict(device=-1), "device"),
-    (dict(steps=2**24, vocab=2**20), "too large"), (dict(steps=2**26, vocab=4), "too large"),
+    (dict(steps=2**24, vocab=2**20), "too large"), (dict(steps=2**28, vocab=4), "too large"),
 ])
 def test_rows_that_the_entries_refuse(bad, text):
     L, r = cabi.lib(), C.byref(_rows(**bad))
