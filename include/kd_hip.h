@@ -389,8 +389,8 @@ typedef struct kd_teacher_rows {
   const void *logits; /* KD_DTYPE_* */
   int32_t slots, id_bytes, dtype;
 } kd_teacher_rows;
-/* Distillation: with 1e-6 <= temperature <= 1e6, q = softmax(teacher / temperature) over a row's filled slots and
- * p = softmax(x / temperature) over the vocabulary,
+/* Distillation: with 1e-6 <= temperature <= 1e6, q = softmax(teacher / temperature) over a row's
+ * filled slots and p = softmax(x / temperature) over the vocabulary,
  *   loss[row] = weight sum_k q_k (log q_k - log p_{id_k})     (a q_k of 0 adds 0)
  *   grad_j    = weight upstream / temperature (p_j - sum_{k: id_k = j} q_k)
  * `weights`, `upstream`: [rows] or NULL (1).  A row of weight 0 or without a filled slot is not
@@ -398,7 +398,8 @@ typedef struct kd_teacher_rows {
  * row of -inf alone: p = 0).  `grad` NULL: the loss alone.  `stats` ([rows][2], or NULL with a
  * loss): maximum and sum of the row, written with a loss; with `loss` NULL they are read, and the
  * call computes the gradient alone (the same inputs as the call that wrote them).  `grad` may be
- * the logits themselves, as in kd_token_scores_grad.  Loss and gradient in one call read a row of up to 32 KiB once. */
+ * the logits themselves, as in kd_token_scores_grad.  Loss and gradient in one call read a row
+ * of up to 64 KiB once, many rows of up to 256 KiB too; longer ones twice. */
 size_t kd_distill_loss_workspace(const kd_frame_rows *rows, int32_t with_grad);
 int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, const float *weights,
                     float temperature, float *loss, float *stats, const float *upstream, void *grad,

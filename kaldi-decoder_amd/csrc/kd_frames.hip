@@ -2,13 +2,22 @@
 // "scores of given tokens" and "distillation"): kernels and their C entries.
 //
 // Everything here works on rows of V logits (f32, f16 or bf16), [batch][steps][V] with strides and
-// optional lengths, the rows that the search itself is handed.  All of it is bound by the bytes of
+// optional lengths, the rows that the search itself is handed.  The operators are bound by the bytes of
 // the logits, so the one rule is that a row is read once: a UNIT -- a whole row, or a segment of a
-// long one -- is loaded into registers with 16-byte loads (NCH per lane, TPU = 64 or 256 threads)
-// and every pass over it (maximum, sums, alternatives, gradient) runs over those registers.  A row
-// of up to 8 KiB is one wave's, up to 32 KiB one workgroup's; a longer one is cut into segments
-// whose partial results (maximum, sums, alternatives) a second kernel joins.
+// long one -- is loaded into the registers of TPU lanes, up to NCH 16-byte loads each, and every pass
+// over it (maximum, sums, alternatives, gradient) runs over those registers.  How rows are dealt out
+// (MakePlan):
+//
+//   row           unit                                  one for all: the steps taken once a row
+//   to 2 KiB      16 lanes, four rows a wave            ... serve four rows
+//   to 8 KiB      a wave                                ... need no barrier
+//   to 32 KiB     a workgroup of 256
+//   to 64 KiB     a workgroup of 512 (values, and loss with gradient)
+//   to 256 KiB    a workgroup of 1024, loss with gradient of many rows: read once, written once
+//   longer, few   segments, whose partial results (maximum, sums, alternatives) a second kernel joins
+//
 // Sums and statistics are f32; logits and gradients are rounded once, on the way in and out.
+// Figures below: one MI355X, kernels in a graph; large copies run at 4.9 TB/s there (read + write).
 
 #include <hip/hip_runtime.h>
 
@@ -592,6 +601,10 @@ __device__ __noinline__ uint64_t KthElement(const SRC src, int *red, float floor
   return Key(val, col);
 }
 
+// (What alternatives cost beside the statistics, 2048 rows of 32768 bf16: 24 us with none, 28 with 1,
+// 31 with 32, 36 with 64; a single row of 262144: 4.9 us with none, 9.3 with 20, most of it the steps that
+// wait for each other in the two kernels.)
+//
 // Puts the unit's K largest elements in order and hands (place, key) to `out`, once per place from
 // some lane; places without an element get key 0.  `threshold`: at least k of the unit's elements
 // reach it, or it is -inf or NaN.  `collect`: Collect or CollectUnit of the elements that reach a value.
@@ -750,6 +763,10 @@ __device__ inline void WriteNoTop(float *v, int32_t *i, float val, int k, int ti
   }
 }
 
+// Statistics, scores and alternatives of a unit: an element costs 1.5 operations for the maximum
+// (v_maximum3 takes two, f16 and bf16 are unpacked first) and 7 (fma, exp2 -- a quarter of the rate --,
+// two sums and their guard), so rows of bf16 keep the vector units as busy as the memory: 268 M elements
+// take 128 us, 4.2 TB/s, where a plain sum over the same bytes by the library runs at 4.0.
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
 __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresKernel(const ScoresArgs a) {
   __shared__ Scratch<TPU> scratch[TOP || TPU > 64 ? kUnits<TPU> : 1];
@@ -932,7 +949,8 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
 // ---- scores of short rows --------------------------------------------------------------------
 // Rows of up to 2 KiB: a wave takes four, 16 lanes (one DPP row) each.  What such a row costs is not
 // its bytes but the steps that are taken once a row -- reductions, threshold, ranking --, and these
-// serve four rows here.
+// serve four rows here: 24000 rows of 500 f32 with 8 alternatives 12.8 us (9.5 without), and 19.5 with a
+// wave a row.  More than 16 alternatives need the 64 groups of a whole wave (21.5 us with 17).
 
 // The k-th largest (k <= 16) of 16 lanes' pairs, in all lanes.
 __device__ inline float RowKthLargest(float a, float b, int k) {
@@ -1147,7 +1165,7 @@ struct ScoresGradArgs {
 
 // dx_j = g_logp ([j = token] - p_j) - g_H p_j (log p_j + H).  With p_j = e_j / s, log p_j = ln 2 t_j -
 // log s (t_j the exponent) that is e_j (A + B t_j) + g_logp [j = token]: A = (-g_logp - g_H (H - log s)) / s,
-// B = -ln 2 g_H / s.
+// B = -ln 2 g_H / s.  Bound by memory: 4096 rows of 65536 bf16 are read and written at 5.9 TB/s.
 template <class T, int NCH, int TPU>
 __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresGradKernel(const ScoresGradArgs a) {
   const int tid = UnitLane<TPU>();
@@ -1328,7 +1346,10 @@ __device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU, 
   for (int i = 0; i < SN; ++i) xs[i] = t.id[i] >= 0 ? T::Load(x + t.id[i]) : 0.0f;
 }
 
-// Whole rows: loss, and with GRAD the gradient from the registers that the statistics were taken of.
+// Whole rows: loss, and with GRAD the gradient from the registers that the statistics were taken of:
+// 4096 rows of 131072 bf16 in 467 us, 4.6 TB/s of one read and one write, where statistics and gradient
+// in two kernels, three passes over memory, take 628.  (A row of 256 KiB fills half a CU's registers, so
+// its loads, sums and stores do not overlap with another's on the same CU; other CUs' do.)
 template <class T, int NCH, int TPU, int SN, bool GRAD>
 __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void DistillKernel(const DistillArgs a) {
   __shared__ TeacherList<TPU, SN> lists[kUnits<TPU>];
@@ -1497,8 +1518,16 @@ int Launch(void (*kernel)(ARGS), uint32_t blocks, const ARGS &args, void *stream
 
 int64_t ElemBytes(int dtype) { return dtype == KD_DTYPE_F32 ? 4 : 2; }
 
-// How rows are dealt out (the comment at the top of this file): TPU threads a unit, up to NCH 16-byte
-// loads each.
+// How rows are dealt out: TPU lanes a unit, up to NCH 16-byte loads each.  Both sides of each rule, in
+// us (D: loss and gradient of bf16 rows; S: scores with 20 alternatives):
+//   whole to 64 KiB         S 1 x 32768 7.1, in segments 10.6; D 8 x 32768 10.3 and 12.7; D 4096 x 32768
+//                           116 and 184
+//   1024 lanes, 128 KiB     D 64 x 65536 15.5, in segments 17.5; 16 x 65536 13.7 and 13.3; 4096 x 65536 219 and 338
+//   1024 lanes, 256 KiB     D 256 x 131072 33.5, in segments 44; 128 x 131072 26.8 and 27.4; 64: 24 and 21.5
+//                           (values alone are read once either way: 512 x 131072 41.7 and 29.4)
+//   smaller segments for    S 1 x 262144 9.4 with 64 units, 9.7 with 16; D 1 x 131072 12.6 and 14.3; but the
+//   few rows                joining kernel holds at most kHeld x 256 alternatives in registers (64
+//                           alternatives: 14.1 with 32 units, 18.9 with 64)
 struct Plan {
   int tpu, nch, seg_len, nseg;
 };
@@ -1665,7 +1694,9 @@ size_t kd_token_scores_workspace(const kd_frame_rows *rows, int32_t top) {
   Rows r;
   Plan p;
   int64_t n;
-  if (top < 0 || CheckRows(rows, kValues, &r, &p, &n, top, top <= kShortTop) || top > kMaxTop || p.nseg == 1) return 0;
+  if (top < 0 || top > kMaxTop || Guarded([&] { return CheckRows(rows, kValues, &r, &p, &n, top, top <= kShortTop); }) ||
+      p.nseg == 1)
+    return 0;
   const size_t units = static_cast<size_t>(n) * p.nseg;
   return Align(units * sizeof(Partial)) + units * top * sizeof(uint64_t);
 }
@@ -1751,7 +1782,8 @@ size_t kd_distill_loss_workspace(const kd_frame_rows *rows, int32_t with_grad) {
   Rows r;
   Plan p;
   int64_t n;
-  if (CheckRows(rows, with_grad ? kFused : kValues, &r, &p, &n, 0, false) || p.nseg == 1) return 0;
+  if (Guarded([&] { return CheckRows(rows, with_grad ? kFused : kValues, &r, &p, &n, 0, false); }) || p.nseg == 1)
+    return 0;
   return Align(static_cast<size_t>(n) * p.nseg * sizeof(Partial)) + Align(static_cast<size_t>(n) * 8);
 }
 

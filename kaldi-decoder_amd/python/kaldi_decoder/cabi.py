@@ -471,7 +471,8 @@ class Batch:
         logits they are the log_softmax of (any type frames.token_scores takes).  `tokens` int32 [B, T]:
         the column that each frame of the best path took -- LogLikelihood(frame, ilabel) reads column
         ilabel - 1 (csrc/decodable-ctc.cc:22-31) --, -1 behind its end; `scores`: frames.TokenScores of
-        them, with `top` alternatives a frame."""
+        them, with `top` alternatives a frame.  For batches that give best paths (not LatticeBatch: an
+        error, as best_paths is), decoded from frame 0 on."""
         import torch
         from . import frames
         if logits.dim() != 3 or logits.shape[0] != self.batch:

@@ -79,20 +79,21 @@ def token_scores_grad(logits, scores, tokens=None, lengths=None, grad_logp=None,
 
 def distill_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, lengths=None):
     """Per row, weight * KL(q || p) over the tokens a teacher lists: q = softmax(teacher_logits /
-    temperature) over the row's list, p = softmax(logits / temperature) over the vocabulary, 1e-6 <= temperature <= 1e6.
+    temperature) over the row's list, p = softmax(logits / temperature) over the vocabulary;
+    1e-6 <= temperature <= 1e6.
 
     `teacher_ids` (int32 or int64) and `teacher_logits` (float32, float16, bfloat16; log-probabilities
     serve as well) [..., K], K <= 256; an id outside [0, V), such as -1, marks an empty slot, one that
     is listed twice counts twice.  `weights` float32, shape logits.shape[:-1]: rows of weight 0, rows
     without a listed token and rows behind `lengths` are not read (loss 0, gradient 0).  The loss
-    (float32, shape logits.shape[:-1]) is differentiable in the logits alone.  Where the weights are all that scales it
-    (a mean: weights of 1 / rows), distill_loss_and_grad does the work of both passes in one."""
+    (float32, shape logits.shape[:-1]) is differentiable in the logits alone.  Where the weights are all
+    that scales it (a mean: weights of 1 / rows), distill_loss_and_grad does the work of both passes in one."""
     return _frames.distill_loss(logits, teacher_ids, teacher_logits, weights, temperature, _tensors(logits, lengths))
 
 
 def distill_loss_and_grad(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, lengths=None, out=None):
     """(loss, gradient of loss.sum() in the logits): distill_loss and its backward pass in one call,
-    which reads rows of up to 32 KiB once.  The gradient goes to `out` (the logits' shape and dtype,
+    which reads rows of up to 64 KiB (many rows of up to 256 KiB) once.  The gradient goes to `out` (the logits' shape and dtype,
     rows that do not overlap; `logits` itself will do) or to a new tensor."""
     return _frames.distill_loss_and_grad(logits, teacher_ids, teacher_logits, weights, temperature,
                                          _tensors(logits, lengths), out)

@@ -4,15 +4,16 @@ be from them.  Rows are handled one list at a time, on the CPU.
 Error bounds.  u = 2^-24 is half a step of f32.  With d_j = x_j - m, e_j = exp(d_j / t):
  * d_j carries u |d_j|, its product with log2(e) / t twice u |d_j / t| more (product and constant),
    exp2 one step (2 u): e_j is off by u (3 |d_j| / t + 2) of itself.
- * a sum of e_j: a lane adds at most 64 of them one by one, then 6 + 2 levels join lanes and waves and
-   at most 8 + nseg / 256 join segments: CHAIN = 96 roundings cover it (rows up to 2^20), and s is off
-   by S = u (CHAIN + E[3 |d| / t + 2]) of itself, with E over p.
+ * a sum of e_j: a lane adds at most 128 of them one by one (64, but for loss and gradient of many rows
+   of 128 to 256 KiB), then 6 levels join lanes, at most 16 waves follow one by one and at most
+   8 + 6 + 4 steps join segments: CHAIN = 168 roundings cover it, and s is off by
+   S = u (CHAIN + E[3 |d| / t + 2]) of itself, with E over p.
  * log s: S, and 2 u |log s| of its own (the library's logarithm is within one step).
 """
 import torch
 
 U = 2.0 ** -24
-CHAIN = 96
+CHAIN = 168
 TINY = 1e-37  # f32 results below 2^-126 may be flushed
 
 

@@ -296,6 +296,69 @@ def test_gradient_over_the_logits(frames, dtype, v):
     assert torch.equal(mine, want)
 
 
+@pytest.mark.parametrize("dtype,n,v", [("f32", 40, 20001), ("bf16", 33, 65536), ("f16", 32, 40003), ("f32", 130, 40001),
+                                       ("bf16", 128, 131072), ("f16", 129, 70001)])
+def test_distillation_of_many_long_rows(frames, dtype, n, v):
+    """Enough rows for a workgroup of 1024 to take each whole (80 to 256 KiB): by the oracle, and next to
+    the same rows a few at a time, which are cut into segments."""
+    dt = DTYPES[dtype]
+    x, dev = _logits(n, v, dt, v, pad=v % 2)
+    g = torch.Generator().manual_seed(n)
+    ids = torch.stack([torch.randperm(v, generator=g)[:40] for _ in range(n)])
+    ids[1, 1], ids[3, 2], ids[9] = ids[1, 0], -1, -1
+    u, w = torch.randn(n, 40, generator=g) * 2, torch.rand(n, generator=g) + 0.5
+    w[10] = 0
+    loss, grad = frames.distill_loss_and_grad(dev, ids.cuda(), u.cuda(), w.cuda(), 2.0)
+    mine = dev.clone()
+    loss2, grad2 = frames.distill_loss_and_grad(mine, ids.cuda(), u.cuda(), w.cuda(), 2.0, out=mine)
+    assert torch.equal(loss, loss2) and torch.equal(grad, grad2) and grad2.data_ptr() == mine.data_ptr()
+    few, few_grad = frames.distill_loss_and_grad(dev[:20], ids[:20].cuda(), u[:20].cuda(), w[:20].cuda(), 2.0)
+    for r in list(range(20)) + [n - 1]:
+        (ref, gr), (tol, tol_g) = frames_ref.row_distill(x[r], ids[r].tolist(), u[r].double().tolist(), w[r].item(), 2.0)
+        tol_g = tol_g + half_step(dt) * (gr.abs() + tol_g) + (2.0 ** -25 if dt == torch.float16 else 0)
+        for one, one_grad in ((loss, grad),) + (((few, few_grad),) if r < 20 else ()):
+            assert _close(one[r].item(), ref, tol + frames_ref.U * abs(ref) if abs(ref) < INF else 0), (r, one[r].item(), ref)
+            assert ((one_grad[r].cpu().double() - gr).abs() <= tol_g).all(), r
+
+
+def test_many_rows_and_the_longest(frames):
+    """Three million rows of four; one row of 2^24 columns, with ties at the last places."""
+    x = torch.randn(3000000, 4).cuda()
+    tokens = torch.randint(0, 4, (3000000,)).cuda()
+    sc = frames.token_scores(x, tokens, top=2)
+    lp = torch.log_softmax(x.double(), -1)
+    # (four terms, |d| < 12: u (4 + 3 * 12 + 2 + 4 * 12) bounds logp, rounded up)
+    tol = 100 * frames_ref.U
+    assert (sc.logp - lp.gather(-1, tokens[:, None]).squeeze(-1)).abs().max() <= tol
+    assert (sc.entropy + (lp.exp() * lp).sum(-1)).abs().max() <= 4 * tol
+    order = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :2]
+    assert torch.equal(sc.top_ids.long(), order)
+    assert (sc.top_logp - lp.gather(-1, order)).abs().max() <= tol
+    v = 1 << 24
+    for dt in (torch.float32, torch.bfloat16):
+        x = torch.randn(1, v).to(dt)
+        x[0, -1] = 9.0
+        tokens = torch.tensor([v - 1])
+        _check_scores(frames.token_scores(x.cuda(), tokens.cuda(), top=64), x, tokens, 64)
+        ids, u = torch.tensor([[v - 1, 0, 5, v // 2]]), torch.randn(1, 4)
+        loss, g = frames.distill_loss_and_grad(x.cuda(), ids.cuda(), u.cuda())
+        (ref, gr), (tol, tol_g) = frames_ref.row_distill(x[0], ids[0].tolist(), u[0].double().tolist(), 1.0, 1.0)
+        assert abs(loss.item() - ref) <= tol + frames_ref.U * abs(ref)
+        assert ((g[0].cpu().double() - gr).abs() <= tol_g + half_step(dt) * (gr.abs() + tol_g)).all()
+
+
+def test_written_in_place_is_noticed(frames):
+    """A graph that saved the logits refuses to go backward once a gradient was written over them."""
+    x = torch.randn(3, 50).cuda()
+    leaf = x.clone().requires_grad_()
+    y = leaf * 1.0
+    ids, u = torch.zeros(3, 1, dtype=torch.int32).cuda(), torch.zeros(3, 1).cuda()
+    loss = frames.distill_loss(y, ids, u)
+    frames.distill_loss_and_grad(y.detach(), ids, u, out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
 def test_gradients_against_differences(frames):
     """Directional derivatives by central differences of the forward kernels.  Along v, |v| <= 1/2, the
     third derivative of logp is a third cumulant of v: at most 1; the entropy's a joint cumulant of
