@@ -1295,16 +1295,17 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU, SN> &t, Tea
   UnitSync<TPU>();
 }
 
-// sum_k q_k (log q_k - log p_k), log p_k = (x_k - m) / temperature - ls; xs: the students' logits at the slots.
+// w sum_k q_k (log q_k - log p_k), log p_k = (x_k - m) / temperature - ls; xs: the students' logits at the slots.
 template <int TPU, int SN>
-__device__ inline float Divergence(const DistillArgs &a, const Slots<TPU, SN> &t, const float (&xs)[SN],
-                                   float m, float ls, float *red) {
+__device__ inline float Divergence(const DistillArgs &a, const Slots<TPU, SN> &t, const float (&xs)[SN], float m,
+                                   float ls, float w, float *red) {
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < SN; ++i) {
-    // (the logit's product is formed with q / temperature: (lowest - m) / temperature alone may overflow)
-    const float d = xs[i] - Base(m), each = (t.u[i] - t.log_usum) + ls;
-    if (t.id[i] >= 0 && t.q[i] != 0.0f) sum += fmaf(t.q[i], each, -(t.q[i] * a.inv_t) * d);
+    // (a logit of the type's lowest value: what it is multiplied by is formed first, or the product of
+    // two of the factors overflows where that of all does not)
+    const float d = xs[i] - Base(m), each = (t.u[i] - t.log_usum) + ls, wq = w * t.q[i];
+    if (t.id[i] >= 0 && t.q[i] != 0.0f) sum += fmaf(wq, each, -(wq * a.inv_t) * d);
   }
   return UnitSum<TPU>(sum, red);
 }
@@ -1399,9 +1400,9 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void Distill
   }
   s0 = UnitSum<TPU>(s0, list.red[3]) * __builtin_amdgcn_exp2f(-exponent.delta);
   const float ls = LogSum(s0);
-  const float loss = Divergence<TPU, SN>(a, t, xs, m, ls, list.red[4]);
+  const float loss = Divergence<TPU, SN>(a, t, xs, m, ls, w, list.red[4]);
   if (tid == 0) {
-    if (a.loss) a.loss[u.row] = w * loss;
+    if (a.loss) a.loss[u.row] = loss;
     if (a.stats) {
       a.stats[2 * static_cast<size_t>(u.row)] = m;
       a.stats[2 * static_cast<size_t>(u.row) + 1] = s0;
@@ -1436,10 +1437,10 @@ __global__ __launch_bounds__(kBlock) void DistillJoinKernel(const DistillArgs a)
   if (t.any) {
     float s1;
     JoinPartials(part, mine, a.r.nseg, a.k2, red, &m, &s0, &s1);
-    loss = Divergence<kBlock, 1>(a, t, xs, m, LogSum(s0), list.red[4]);
+    loss = Divergence<kBlock, 1>(a, t, xs, m, LogSum(s0), w, list.red[4]);
   }
   if (tid == 0) {
-    if (a.loss) a.loss[u.row] = t.any ? w * loss : 0.0f;
+    if (a.loss) a.loss[u.row] = t.any ? loss : 0.0f;
     a.stats[2 * static_cast<size_t>(u.row)] = m;
     a.stats[2 * static_cast<size_t>(u.row) + 1] = s0;
   }
