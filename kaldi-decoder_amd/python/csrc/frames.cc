@@ -7,6 +7,7 @@
 // same row: 4.3), and 15 through ctypes.  With a gradient through autograd 35 us (a product of two
 // tensors and its gradient: 27), and 120.
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -117,6 +118,7 @@ Tensor GradOut(const OptTensor &out, const Tensor &x) {
   TORCH_CHECK_VALUE(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->device() == x.device(),
                     "out must have the logits' shape, dtype and device");
   TORCH_CHECK_VALUE(out->stride(-1) == 1 || out->size(-1) == 1, "out needs unit stride over the last (V) dimension");
+  at::assert_no_partial_overlap(*out, x);  // (the logits themselves will do)
   // (written in place: a graph that saved it must notice)
   out->unsafeGetTensorImpl()->bump_version();
   return *out;

@@ -347,6 +347,50 @@ def test_many_rows_and_the_longest(frames):
         assert ((g[0].cpu().double() - gr).abs() <= tol_g + half_step(dt) * (gr.abs() + tol_g)).all()
 
 
+@pytest.mark.parametrize("v", [30, 700, 5000, 20000, 50000])
+def test_autograd_of_padded_batches(frames, v):
+    """Graphs over [B, T, V] with lengths from the host, without tokens, with alternatives; rows that are
+    not read (behind the lengths, of weight 0) may hold anything."""
+    lengths = [4, 0, 2]
+    x = torch.randn(3, 4, v).cuda()
+    x[0, 3] = x[2, 2:] = x[1] = float("nan")
+    lengths[0] = 3
+    tokens = torch.randint(0, v, (3, 4)).cuda()
+    leaf = x.clone().requires_grad_()
+    up = torch.randn(3, 4).cuda()
+    sc = frames.token_scores(leaf, None, top=3, lengths=lengths)
+    assert sc.logp is None and sc.entropy.requires_grad and not sc.top_logp.requires_grad and not sc.stats.requires_grad
+    got, = torch.autograd.grad(sc.entropy, leaf, up)
+    want = frames.token_scores_grad(x, frames.token_scores(x, lengths=lengths), None, torch.tensor(lengths), None, up)
+    assert torch.equal(got, want) and got.isfinite().all() and got[1].eq(0).all() and got[0, :3].ne(0).any()
+    sc = frames.token_scores(leaf, tokens, top=3, lengths=lengths)
+    assert sc.logp[1].eq(0).all() and sc.logp.isfinite().all()
+    got, = torch.autograd.grad((sc.logp * up).sum() + sc.entropy.sum(), leaf)
+    want = frames.token_scores_grad(x, sc, tokens, lengths, up, torch.ones(3, 4).cuda())
+    assert torch.equal(got, want)
+    ids, u, w = torch.randint(0, v, (3, 4, 9)).cuda(), torch.randn(3, 4, 9).cuda(), torch.rand(3, 4).cuda()
+    loss = frames.distill_loss(leaf, ids, u, w, 1.5, lengths)
+    got, = torch.autograd.grad((loss * up).sum(), leaf)
+    loss2, one = frames.distill_loss_and_grad(x, ids, u, w, 1.5, lengths)
+    # (upstream gradients are multiplied in before the one rounding)
+    assert (got - one * up[..., None]).abs().max() <= 1e-6 and loss.isfinite().all() and loss2.isfinite().all()
+    skip = torch.where(torch.isnan(x).any(-1), 0.0, w.double()).float()
+    loss3, three = frames.distill_loss_and_grad(x, ids, u, skip, 1.5)
+    assert torch.equal(loss3, loss2) and torch.equal(three, one)
+
+
+def test_a_gradient_may_not_lie_across_the_logits(frames):
+    base = torch.randn(5 * 40 + 3).cuda()
+    x, out = base[:200].view(5, 40), base[3:].view(5, 40)
+    ids, u = torch.zeros(5, 1, dtype=torch.int32).cuda(), torch.zeros(5, 1).cuda()
+    with pytest.raises(RuntimeError, match="memory location"):
+        frames.distill_loss_and_grad(x, ids, u, out=out)
+    wide = torch.randn(5, 80).cuda()  # (side by side in one storage: apart)
+    _, want = frames.distill_loss_and_grad(wide[:, :40].clone(), ids, u)
+    _, got = frames.distill_loss_and_grad(wide[:, :40], ids, u, out=wide[:, 40:])
+    assert torch.equal(got, want)
+
+
 def test_written_in_place_is_noticed(frames):
     """A graph that saved the logits refuses to go backward once a gradient was written over them."""
     x = torch.randn(3, 50).cuda()
