@@ -221,33 +221,40 @@ __device__ inline void NewPass(U4 (&r)[NCH]) {
 __device__ inline float Max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ inline float Min(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 
-template <int CTRL, int ROW_MASK = 0xf, int BANK_MASK = 0xf>
-__device__ inline int DppI(int old, int v) {
-  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROW_MASK, BANK_MASK, false);
-}
-template <int CTRL, int ROW_MASK = 0xf, int BANK_MASK = 0xf>
+template <int CTRL, int ROW_MASK, int BANK_MASK = 0xf>
 __device__ inline float Dpp(float old, float v) {
-  return __int_as_float(DppI<CTRL, ROW_MASK, BANK_MASK>(__float_as_int(old), __float_as_int(v)));
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROW_MASK, BANK_MASK,
+                                                    false));
+}
+// The same where every lane takes part: lanes without a source get 0.  (Nothing is kept of an old value,
+// so the move becomes an operand of what uses it.)
+template <int CTRL>
+__device__ inline int MoveI(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ inline float Move(float v) {
+  return __int_as_float(MoveI<CTRL>(__float_as_int(v)));
 }
 // Over 16 lanes (a DPP row), by rotations: every lane has the result.
 constexpr int kRowRor = 0x120;
 __device__ inline float RowMax(float v) {
-  v = Max(v, Dpp<kRowRor + 8>(v, v));
-  v = Max(v, Dpp<kRowRor + 4>(v, v));
-  v = Max(v, Dpp<kRowRor + 2>(v, v));
-  return Max(v, Dpp<kRowRor + 1>(v, v));
+  v = Max(v, Move<kRowRor + 8>(v));
+  v = Max(v, Move<kRowRor + 4>(v));
+  v = Max(v, Move<kRowRor + 2>(v));
+  return Max(v, Move<kRowRor + 1>(v));
 }
 __device__ inline float RowSum(float v) {
-  v += Dpp<kRowRor + 8>(v, v);
-  v += Dpp<kRowRor + 4>(v, v);
-  v += Dpp<kRowRor + 2>(v, v);
-  return v + Dpp<kRowRor + 1>(v, v);
+  v += Move<kRowRor + 8>(v);
+  v += Move<kRowRor + 4>(v);
+  v += Move<kRowRor + 2>(v);
+  return v + Move<kRowRor + 1>(v);
 }
 __device__ inline int RowSum(int v) {
-  v += DppI<kRowRor + 8>(v, v);
-  v += DppI<kRowRor + 4>(v, v);
-  v += DppI<kRowRor + 2>(v, v);
-  return v + DppI<kRowRor + 1>(v, v);
+  v += MoveI<kRowRor + 8>(v);
+  v += MoveI<kRowRor + 4>(v);
+  v += MoveI<kRowRor + 2>(v);
+  return v + MoveI<kRowRor + 1>(v);
 }
 // Over a wave: rows 1 and 3 take over what row 0 and 2 have, then rows 2 and 3; lane 63 has all.
 __device__ inline float Lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
@@ -382,7 +389,7 @@ __device__ inline int ColumnOf(uint64_t key) { return static_cast<int>(~static_c
 __device__ inline float Keep(float v, float o, bool below) { return below ? Max(v, o) : Min(v, o); }
 template <int CTRL>
 __device__ inline float Exchange(float v, bool below) {
-  return Keep(v, Dpp<CTRL>(v, v), below);
+  return Keep(v, Move<CTRL>(v), below);
 }
 __device__ inline float Exchange4(float v) {  // lane ^ 4: the lane 4 further or 4 before
   const float up = Dpp<0x104, 0xf, 0x5>(v, v);
@@ -957,7 +964,7 @@ __device__ inline float RowKthLargest(float a, float b, int k) {
   a = RowSort(a);
   b = RowSort(b);
   // the 16 largest of both are the larger of the l-th and the (15 - l)-th: a bitonic sequence
-  a = RowMerge(Max(a, Dpp<0x140>(b, b)));
+  a = RowMerge(Max(a, Move<0x140>(b)));
   return OfLane(a, (threadIdx.x & 48) + k - 1);
 }
 
@@ -989,10 +996,10 @@ __device__ __noinline__ uint64_t ShortKthElement(const typename T::Store *p, int
 }
 // Sum over a row's lanes up to and with one's own.
 __device__ inline int RowPrefix(int v) {
-  v += DppI<0x111>(0, v);  // row_shr:1
-  v += DppI<0x112>(0, v);
-  v += DppI<0x114>(0, v);
-  return v + DppI<0x118>(0, v);
+  v += MoveI<0x111>(v);  // row_shr:1
+  v += MoveI<0x112>(v);
+  v += MoveI<0x114>(v);
+  return v + MoveI<0x118>(v);
 }
 
 template <class T, int NCH, bool TOP>
