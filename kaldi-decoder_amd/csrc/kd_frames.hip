@@ -1240,8 +1240,7 @@ template <int TPU, int SN>
 constexpr int kListed = TPU * SN < kMaxSlots ? TPU * SN : kMaxSlots;
 template <int TPU, int SN>
 struct TeacherList {
-  int id[kListed<TPU, SN>];
-  float q[kListed<TPU, SN>];
+  int2 slot[kListed<TPU, SN>];  // id, and the bits of q
   float red[5][TPU < 64 ? 1 : TPU / 64];
 };
 template <int TPU, int SN>
@@ -1295,8 +1294,7 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU, SN> &t, Tea
     t.q[i] = t.q[i] / sum;
     const int k = i * TPU + tid;
     if (k < a.slots) {
-      list.id[k] = t.id[i];
-      list.q[k] = t.q[i];
+      list.slot[k] = int2{t.id[i], __float_as_int(t.q[i])};
     }
   }
   UnitSync<TPU>();
@@ -1334,17 +1332,25 @@ __device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, con
     for (int j = 0; j < T::kVec; ++j) g[j] = scale * __builtin_amdgcn_exp2f(exponent(T::Get(v, j)));
   });
   UnitSync<TPU>();
+  bool mine[SN], any = false;
+  float q[SN];
 #pragma unroll
   for (int i = 0; i < SN; ++i) {
-    if (i * TPU >= a.slots) break;
     const int at = t.id[i] - u.lo;
-    const bool mine = t.id[i] >= 0 && at >= 0 && at < u.n;
-    if (__ballot(mine)) {
-      float q = 0.0f;
-      for (int k = 0; k < a.slots; ++k) q += list.id[k] == t.id[i] ? list.q[k] : 0.0f;
-      if (mine) dx[at] = T::Round(coef * (__builtin_amdgcn_exp2f(exponent(xs[i])) * inv - q));
-    }
+    mine[i] = t.id[i] >= 0 && at >= 0 && at < u.n;
+    any |= mine[i];
+    q[i] = 0.0f;
   }
+  if (!__ballot(any)) return;
+#pragma unroll 4
+  for (int k = 0; k < a.slots; ++k) {
+    const int2 slot = list.slot[k];
+#pragma unroll
+    for (int i = 0; i < SN; ++i) q[i] += slot.x == t.id[i] ? __int_as_float(slot.y) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < SN; ++i)
+    if (mine[i]) dx[t.id[i] - u.lo] = T::Round(coef * (__builtin_amdgcn_exp2f(exponent(xs[i])) * inv - q[i]));
 }
 
 // The students' logits at a lane's slots.
