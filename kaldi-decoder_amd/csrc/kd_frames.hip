@@ -132,10 +132,10 @@ template <int TPU>
 constexpr int kThreads = TPU < kBlock ? kBlock : TPU;  // of a workgroup
 // Waves a SIMD that a kernel is compiled for (1: as many as its registers allow).  Units of 512 lanes
 // take two a SIMD, so 68 registers instead of 64 would cost one unit in four (40.4 instead of 43.2 us
-// for 2048 rows of 32768 bf16 with 64 alternatives); the others lose a wave slot in eight at most, and
-// more by spilling.
+// for 2048 rows of 32768 bf16 with 64 alternatives); units of 16 lanes hold 16 addresses a lane unless
+// told not to (24.7 instead of 25.6 us for the loss and gradient of 24000 rows of 500 with 32 slots).
 template <int TPU, int NCH>
-constexpr int kOccupancy = TPU == 512 || (TPU == 1024 && NCH <= 8) ? 8 : 1;
+constexpr int kOccupancy = TPU == 16 || TPU == 512 || (TPU == 1024 && NCH <= 8) ? 8 : 1;
 template <int TPU>
 __device__ inline int UnitLane() {
   return TPU < kBlock ? (threadIdx.x & (TPU - 1)) : threadIdx.x;
