@@ -1539,9 +1539,10 @@ int64_t ElemBytes(int dtype) { return dtype == KD_DTYPE_F32 ? 4 : 2; }
 //   1024 lanes, 128 KiB     D 64 x 65536 15.5, in segments 17.5; 16 x 65536 13.7 and 13.3; 4096 x 65536 219 and 338
 //   1024 lanes, 256 KiB     D 256 x 131072 33.5, in segments 44; 128 x 131072 26.8 and 27.4; 64: 24 and 21.5
 //                           (values alone are read once either way: 512 x 131072 41.7 and 29.4)
-//   smaller segments for    S 1 x 262144 9.4 with 64 units, 9.7 with 16; D 1 x 131072 12.6 and 14.3; but the
-//   few rows                joining kernel holds at most kHeld x 256 alternatives in registers (64
-//                           alternatives: 14.1 with 32 units, 18.9 with 64)
+//   smaller segments for    S 8 x 131072 9.9 with 256 units and more, 10.6 with 64; D 8 x 131072 13.3 and 14.8; S 1 x
+//   few rows                262144 9.3 and 9.4 (from 1024 units on the joining kernel's share grows: 16 x 131072
+//                           10.1 with 512, 10.8 with 1024).  That kernel holds at most kHeld x 256
+//                           alternatives in registers (1 x 262144 with 64: 14.1 with 32 units, 18.9 with 64)
 struct Plan {
   int tpu, nch, seg_len, nseg;
 };
@@ -1563,7 +1564,7 @@ Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what, int top, boo
   if (what == kFused && bytes <= 262144 && rows >= 128) return {1024, 16, whole, 1};
   Plan p{kBlock, 8, 0, 0};
   int64_t cap = 32768;
-  while (cap > 4096 && rows * ((bytes + cap - 1) / cap) < 64 && 2 * top * ((bytes + cap - 1) / cap) <= kHeld * kBlock)
+  while (cap > 4096 && rows * ((bytes + cap - 1) / cap) < 256 && 2 * top * ((bytes + cap - 1) / cap) <= kHeld * kBlock)
     cap /= 2;
   cap /= ElemBytes(dtype);
   p.nseg = static_cast<int>((vocab + cap - 1) / cap);
