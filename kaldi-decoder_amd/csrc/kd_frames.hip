@@ -1304,13 +1304,18 @@ __device__ inline void SoftmaxSlots(const DistillArgs &a, Slots<TPU, SN> &t, Tea
 template <int TPU, int SN>
 __device__ inline float Divergence(const DistillArgs &a, const Slots<TPU, SN> &t, const float (&xs)[SN], float m,
                                    float ls, float w, float *red) {
+  // No product of two or three of the factors stays in f32's range (a logit of the type's lowest value times
+  // 1 / temperature, a small weight times a small q -- and that product must not be 0 where the student rules
+  // the token out, d = -inf).  So w is taken apart, (log q - log p) carries 2^-64 and q 2^40, exactly: the
+  // first is below 2^85 then and the second at least 2^-110, and one ldexp rounds the term.
+  const float w40 = __builtin_amdgcn_frexp_mantf(w) * 0x1p40f, inv_t64 = a.inv_t * 0x1p-64f;
+  const int exponent = __builtin_amdgcn_frexp_expf(w) + 24;
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < SN; ++i) {
-    // (a logit of the type's lowest value: what it is multiplied by is formed first, or the product of
-    // two of the factors overflows where that of all does not)
-    const float d = xs[i] - Base(m), each = (t.u[i] - t.log_usum) + ls, wq = w * t.q[i];
-    if (t.id[i] >= 0 && t.q[i] != 0.0f) sum += fmaf(wq, each, -(wq * a.inv_t) * d);
+    const float d = xs[i] - Base(m), each = (t.u[i] - t.log_usum) + ls;
+    if (t.id[i] >= 0 && t.q[i] != 0.0f)
+      sum += __builtin_amdgcn_ldexpf(w40 * t.q[i] * fmaf(-inv_t64, d, each * 0x1p-64f), exponent);
   }
   return UnitSum<TPU>(sum, red);
 }
