@@ -728,7 +728,20 @@ __device__ inline TokenLogit LoadToken(const ScoresArgs &a, uint32_t row, const 
 __device__ inline float Base(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ inline float LogSum(float s0) { return s0 == 0.0f ? 0.0f : logf(s0); }
 
-// s1 = sum e_j log2(e_j): H = log s - ln 2 s1 / s, two terms that are at least 0: nothing cancels.
+// A unit's s0 and s1 = sum e_j log2(e_j) without what the rounding of the exponents' c added to them
+// (Exponent).  The maximum's own e is exp2(delta) exp2(-delta), 1 but for two roundings: with a finite
+// maximum the sum is at least 1 and s1 at most 0, or a row that one token has to itself would give
+// log-probabilities above 0 and entropies below.  (NaN stays.)
+__device__ inline float Corrected0(float s0, float less, float m) {
+  s0 *= less;
+  return m == -INFINITY ? s0 : Max(s0, 1.0f);
+}
+__device__ inline float Corrected1(float s0, float s1, float delta, float less) {
+  return Min(fmaf(-delta, s0, s1) * less, 0.0f);
+}
+
+// H = log s - ln 2 s1 / s, two terms that are at least 0.  (What cancels is within s1: delta s0, where delta is
+// at most 2^-24 of the maximum's own exponent.)
 __device__ inline void WriteRowScores(const ScoresArgs &a, uint32_t row, TokenLogit tok, float m, float s0, float s1) {
   const float ls = LogSum(s0);
   if (a.tokens) a.logp[row] = tok.there ? (tok.x - Base(m)) - ls : 0.0f;
@@ -836,8 +849,8 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresK
     if (ENT) s1 = SumOf<TPU>(s.red[2]);
   }
   const float less = __builtin_amdgcn_exp2f(-exponent.delta);
-  if (ENT) s1 = fmaf(-exponent.delta, s0, s1) * less;
-  s0 *= less;
+  if (ENT) s1 = Corrected1(s0, s1, exponent.delta, less);
+  s0 = Corrected0(s0, less, m);
 
   if (SPLIT) {
     if (tid == 0) a.part[unit] = Partial{m, s0, s1, 0.0f};
@@ -1048,8 +1061,8 @@ __global__ __launch_bounds__(kBlock) void ScoresShortKernel(const ScoresArgs a) 
   s0 = RowSum(s0);
   s1 = RowSum(s1);
   const float less = __builtin_amdgcn_exp2f(-exponent.delta);
-  s1 = fmaf(-exponent.delta, s0, s1) * less;
-  s0 *= less;
+  s1 = Corrected1(s0, s1, exponent.delta, less);
+  s0 = Corrected0(s0, less, m);
   const float ls = LogSum(s0);
   if (l == 0) WriteRowScores(a, row, tok, m, s0, s1);
   if (!TOP) return;
@@ -1416,7 +1429,7 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void Distill
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) s0 += __builtin_amdgcn_exp2f(exponent(T::Get(r[c], j)));
   }
-  s0 = UnitSum<TPU>(s0, list.red[3]) * __builtin_amdgcn_exp2f(-exponent.delta);
+  s0 = Corrected0(UnitSum<TPU>(s0, list.red[3]), __builtin_amdgcn_exp2f(-exponent.delta), m);
   const float ls = LogSum(s0);
   const float loss = Divergence<TPU, SN>(a, t, xs, m, ls, w, list.red[4]);
   if (tid == 0) {

@@ -49,3 +49,28 @@ def test_small_weights_beside_ruled_out_tokens(frames, v, slots, dtype):
                 elif rows[r - len(rows)][0] <= 60:  # (further down q is below 2^-126 and has few bits)
                     # (the slots' terms are rounded once each: the bound's own u |ref|, twice)
                     assert abs(got[r].item() - ref) <= tol + 2 * frames_ref.U * abs(ref), (r, t, got[r].item(), ref)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("v", [40, 500, 1000, 3000, 9000, 20000, 40000, 100000])
+def test_no_probability_above_one(frames, v, dtype):
+    """Rows that one token has almost to itself, at many heights: its own term makes the sum at least 1,
+    so no log-probability is above 0, and no entropy or divergence below."""
+    n = 200
+    x = torch.full((n, v), -INF)
+    x[1::2] = -1.0
+    x[:, 2] = torch.linspace(-130, 130, n)
+    x = x.to(DTYPES[dtype]).cuda()
+    tokens = torch.full((n,), 2, dtype=torch.int32).cuda()
+    for top in (0, 3, 40):
+        sc = frames.token_scores(x, tokens, top=top)
+        assert (sc.stats[:, 1] >= 1).all() and (sc.entropy >= 0).all() and (sc.logp <= 0).all()
+        assert not top or (sc.top_logp <= 0).all()
+    for t in (1.0, 0.7, 3.0):
+        loss, _ = frames.distill_loss_and_grad(x, tokens[:, None], torch.zeros(n, 1).cuda(), None, t)
+        alone = frames.distill_loss(x, tokens[:, None], torch.zeros(n, 1).cuda(), None, t)
+        assert (loss >= 0).all() and (alone >= 0).all()
+    # rows without a finite value, and rows with NaN, are what they were
+    x[0], x[1, 0] = -INF, float("nan")
+    sc = frames.token_scores(x, tokens)
+    assert sc.stats[0].tolist() == [-INF, 0] and sc.entropy[0] == 0 and torch.isnan(sc.stats[1, 1])
