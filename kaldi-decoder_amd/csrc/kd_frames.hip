@@ -1333,6 +1333,13 @@ __device__ inline float Divergence(const DistillArgs &a, const Slots<TPU, SN> &t
   return UnitSum<TPU>(sum, red);
 }
 
+// weight upstream / temperature of a row: the product of two of them may leave f32's range where that of all
+// three does not, so it is formed in 64 bits.
+__device__ inline float GradFactor(const DistillArgs &a, uint32_t row, float w) {
+  const float up = a.upstream ? a.upstream[row] : 1.0f;
+  return static_cast<float>(static_cast<double>(w) * a.inv_t * up);
+}
+
 // Writes a unit's gradient: coef (p_j - sum of the q of the slots that name column j).  The slots'
 // columns are written again behind the others, by one lane each (slots that name one column write
 // the same value).
@@ -1441,7 +1448,7 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void Distill
   }
   if (GRAD) {
     NewPass(r);
-    const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
+    const float coef = GradFactor(a, u.row, w);
     WriteDistillGrad<T, NCH, TPU, SN>(a, u, r, t, xs, list, m, s0, coef, tid);
   }
 }
@@ -1506,7 +1513,7 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void Distill
     return;
   }
   const float m = a.stats[2 * static_cast<size_t>(u.row)], s0 = a.stats[2 * static_cast<size_t>(u.row) + 1];
-  const float coef = w * a.inv_t * (a.upstream ? a.upstream[u.row] : 1.0f);
+  const float coef = GradFactor(a, u.row, w);
   WriteDistillGrad<T, NCH, TPU, SN>(a, u, r, t, xs, list, m, s0, coef, tid);
 }
 

@@ -74,3 +74,23 @@ def test_no_probability_above_one(frames, v, dtype):
     x[0], x[1, 0] = -INF, float("nan")
     sc = frames.token_scores(x, tokens)
     assert sc.stats[0].tolist() == [-INF, 0] and sc.entropy[0] == 0 and torch.isnan(sc.stats[1, 1])
+
+
+def test_factors_of_the_gradient(frames):
+    """weight * upstream / temperature, where the product of two of them leaves float32's range and that
+    of all three does not."""
+    for v in (40, 3000, 20000, 70000):
+        x = torch.randn(4, v, generator=torch.Generator().manual_seed(v))
+        ids, u = torch.tensor([[1, 3]] * 4), torch.zeros(4, 2)
+        w = torch.tensor([1e35, 1e-36, 1.0, 1e-30])
+        up = torch.tensor([1e-36, 1e30, 0.5, 1e30])
+        for t in (1e-4, 1e4):
+            leaf = (x * t).cuda().requires_grad_()
+            loss = frames.distill_loss(leaf, ids.cuda(), (u * t).cuda(), w.cuda(), t)
+            got, = torch.autograd.grad(loss, leaf, up.cuda())
+            for r in range(4):
+                _, gr = frames_ref.row_distill(leaf[r].detach().cpu(), ids[r].tolist(), (u[r] * t).double().tolist(),
+                                               w[r].double().item(), t, up[r].double().item())[0]
+                tol = frames_ref.row_distill(leaf[r].detach().cpu(), ids[r].tolist(), (u[r] * t).double().tolist(),
+                                             w[r].double().item(), t, up[r].double().item())[1][1]
+                assert ((got[r].cpu().double() - gr).abs() <= tol + 2 * frames_ref.U * gr.abs()).all(), (v, r, t)
