@@ -56,6 +56,12 @@ T *Ptr(const OptTensor &t) {
   return t && t->defined() ? static_cast<T *>(t->data_ptr()) : nullptr;
 }
 
+// A tangent of forward-mode differentiation would be dropped without a word, a derivative of 0.
+void NoTangent(const Tensor &t, const char *what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "kaldi_decoder.frames has no forward-mode derivatives, and ",
+                              what, " carries a tangent: detach it");
+}
+
 // Rows of logits [N, V] or [B, T, V] as the C entries take them.
 struct Rows {
   kd_frame_rows r{};
@@ -63,6 +69,7 @@ struct Rows {
   OptTensor lengths;          // (kept alive until the launch)
 
   Rows(const Tensor &x, const OptTensor &len) {
+    NoTangent(x, "the tensor of logits");
     const int dtype = DtypeCode(x);
     TORCH_CHECK_VALUE(x.is_cuda() && dtype >= 0, "logits must be a float32, float16 or bfloat16 CUDA tensor");
     const int64_t dims = x.dim();
@@ -98,6 +105,7 @@ Tensor PerRow(const Tensor &t, const Rows &rows, int64_t tail, const Tensor &x, 
               const char *types) {
   TORCH_CHECK_VALUE(t.defined() && type_ok && t.device() == x.device(), what, " must be a tensor of ", types, " on ",
                     x.device());
+  NoTangent(t, what);
   const int64_t n = static_cast<int64_t>(rows.lead.size());
   bool same = t.dim() == n + (tail ? 1 : 0) && (!tail || t.size(n) == tail);
   for (int64_t i = 0; same && i < n; ++i) same = t.size(i) == rows.lead[i];
@@ -117,6 +125,7 @@ Tensor GradOut(const OptTensor &out, const Tensor &x) {
   if (!out || !out->defined()) return Empty(x.sizes(), x.scalar_type(), x);
   TORCH_CHECK_VALUE(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->device() == x.device(),
                     "out must have the logits' shape, dtype and device");
+  NoTangent(*out, "out");
   TORCH_CHECK_VALUE(out->stride(-1) == 1 || out->size(-1) == 1, "out needs unit stride over the last (V) dimension");
   at::assert_no_partial_overlap(*out, x);  // (the logits themselves will do)
   // (written in place: a graph that saved it must notice)
@@ -277,6 +286,7 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, const Tensor &teacher,
                         const OptTensor &weights, double temperature, const OptTensor &lengths) {
     OptTensor len = lengths && lengths->defined() ? OptTensor(Rows::Lengths(*lengths, x)) : std::nullopt;
+    NoTangent(x, "the tensor of logits");
     TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1, "logits must be a float32, float16 or bfloat16 CUDA tensor");
     std::vector<int64_t> wide(x.sizes().begin(), x.sizes().end());
     wide.back() = 2;

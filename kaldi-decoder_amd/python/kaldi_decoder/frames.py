@@ -15,6 +15,9 @@ that are not on the device yet): they can be captured into a graph.  A backward 
 autograd that is to be captured needs its leaves to have no live graph from outside the capture, as
 any of torch's; `token_scores_grad` and `distill_loss_and_grad` have no such condition.
 
+What is differentiable is so once, backwards: a second derivative (create_graph) and forward mode (a tensor that
+carries a tangent) raise an error.  `token_scores_grad` and `distill_loss_and_grad` are outside autograd altogether.
+
 (The reference leaves all of this to its callers; its DecodableCtc takes log-probabilities,
 csrc/decodable-ctc.cc:28.)
 """

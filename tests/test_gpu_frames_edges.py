@@ -94,3 +94,21 @@ def test_factors_of_the_gradient(frames):
                 tol = frames_ref.row_distill(leaf[r].detach().cpu(), ids[r].tolist(), (u[r] * t).double().tolist(),
                                              w[r].double().item(), t, up[r].double().item())[1][1]
                 assert ((got[r].cpu().double() - gr).abs() <= tol + 2 * frames_ref.U * gr.abs()).all(), (v, r, t)
+
+
+def test_forward_mode_derivatives_are_refused(frames):
+    import torch.autograd.forward_ad as fwd
+    x, ids, u = torch.randn(3, 40).cuda(), torch.zeros(3, 2, dtype=torch.int32).cuda(), torch.randn(3, 2).cuda()
+    sc = frames.token_scores(x, ids[:, 0])
+    up = torch.ones(3).cuda()
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: frames.token_scores(dual(x)), lambda: frames.token_scores(dual(x).requires_grad_()),
+                     lambda: frames.distill_loss(dual(x), ids, u), lambda: frames.distill_loss(x, ids, dual(u)),
+                     lambda: frames.distill_loss(x, ids, u, dual(up)),
+                     lambda: frames.distill_loss_and_grad(dual(x), ids, u),
+                     lambda: frames.token_scores_grad(x, sc, ids[:, 0], None, dual(up))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(frames.token_scores(dual(x).detach()).entropy, sc.entropy)
