@@ -375,8 +375,9 @@ int kd_token_scores(const kd_frame_rows *rows, const void *tokens, int32_t token
                     void *workspace, size_t workspace_bytes, void *stream);
 /* The logits' gradient for upstream gradients of logp and entropy ([rows], either may be NULL: 0):
  *   grad_j = grad_logp ([j = token] - p_j) - grad_entropy p_j (log p_j + entropy)
- * into `grad` (the logits' dtype and shape, strides of its own; rows must not overlap; apart from the
- * logits, or the logits themselves: the gradient is then written over them).  A row of -inf alone gets zeros. */
+ * into `grad` (the logits' dtype and shape, strides of its own; rows must not overlap; no element in the place
+ * of anything that the call reads, but that `grad` may be the logits themselves, pointer and strides: the
+ * gradient is then written over them.  Other overlaps are KD_E_INVALID).  A row of -inf alone gets zeros. */
 int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t token_bytes,
                          const float *stats, const float *entropy, const float *grad_logp,
                          const float *grad_entropy, void *grad, int64_t grad_batch_stride,

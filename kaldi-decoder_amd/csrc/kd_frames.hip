@@ -25,6 +25,7 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "kd_device.h"
@@ -1629,22 +1630,109 @@ int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64
   return KD_OK;
 }
 
-// A gradient's rows must not lie over each other.
-int CheckGrad(const kd_frame_rows *r, void *dx, int64_t batch_stride, int64_t row_stride, GradOut *o) {
+// Rows in memory, in bytes from `base` on: n[1] groups, s[1] apart, of n[0] runs of `width`, s[0] apart.
+// (Strides may be anything: 128 bits hold what they add up to.)
+typedef __int128 Wide;
+struct Region {
+  uintptr_t base;
+  int64_t n[2];
+  Wide s[2], width;
+
+  Region(const void *p, const kd_frame_rows *r, int64_t batch_stride, int64_t row_stride)
+      : base(reinterpret_cast<uintptr_t>(p)), n{r->steps, r->batch}, width(r->vocab * ElemBytes(r->dtype)) {
+    s[0] = Wide(row_stride) * ElemBytes(r->dtype);
+    s[1] = Wide(batch_stride) * ElemBytes(r->dtype);
+    for (int i = 0; i < 2; ++i)
+      if (n[i] <= 1) s[i] = 0;  // (a stride that is never taken)
+    if (n[0] <= 1 || (n[1] > 1 && s[0] > s[1])) {
+      std::swap(n[0], n[1]);
+      std::swap(s[0], s[1]);
+    }
+  }
+  // Runs that touch or lie over each other are one.
+  void Merge() {
+    for (int i = 0; i < 2 && n[0] > 1 && s[0] <= width; ++i) {
+      width += (n[0] - 1) * s[0];
+      n[0] = n[1];
+      s[0] = s[1];
+      n[1] = 1;
+      s[1] = 0;
+    }
+  }
+  Wide Inner() const { return width + (n[0] - 1) * s[0]; }  // of a group
+  Wide Span() const { return Inner() + (n[1] - 1) * s[1]; }
+  bool Same(const Region &o) const {
+    return base == o.base && n[0] == o.n[0] && n[1] == o.n[1] && s[0] == o.s[0] && s[1] == o.s[1] && width == o.width;
+  }
+};
+Wide FloorDiv(Wide a, Wide b) { return a / b - (a % b < 0); }  // (b > 0)
+// First and last of the 0 <= i < n with lo < i * s + width and i * s < hi; none: first > last.
+void Hits(Wide lo, Wide hi, Wide s, Wide width, int64_t n, Wide *first, Wide *last) {
+  *first = n > 1 ? std::max(FloorDiv(lo - width, s) + 1, Wide(0)) : Wide(lo < width ? 0 : 1);
+  *last = n > 1 ? std::min(FloorDiv(hi - 1, s), Wide(n - 1)) : Wide(hi > 0 ? 0 : -1);
+}
+// Whether bytes [at, at + bytes) meet any run of `g`, whose runs and groups lie one behind the other.
+bool Meets(const Region &g, uintptr_t at, Wide bytes) {
+  if (bytes <= 0) return false;
+  const Wide lo = Wide(at) - Wide(g.base), hi = lo + bytes;
+  Wide first, last, run, end;
+  Hits(lo, hi, g.s[1], g.Inner(), g.n[1], &first, &last);
+  if (first != last) return first < last;  // (none, or all that is between two groups' starts)
+  Hits(lo - first * g.s[1], hi - first * g.s[1], g.s[0], g.width, g.n[0], &run, &end);
+  return run <= end;
+}
+// Whether any byte of `x` is one of `g`, whose runs and groups lie one behind the other.
+bool Meets(const Region &g, const Region &x) {
+  if (Wide(x.base) + x.Span() <= Wide(g.base) || Wide(g.base) + g.Span() <= Wide(x.base)) return false;
+  if (g.n[0] == x.n[0] && g.n[1] == x.n[1] && g.s[0] == x.s[0] && g.s[1] == x.s[1] && g.width == x.width) {
+    // side by side in one tensor: some whole number of strides must lead from one to within the other
+    const Wide delta = Wide(x.base) - Wide(g.base), inner = g.Inner();
+    Wide j = 0, last = 0;
+    if (g.n[1] > 1) {
+      j = std::max(FloorDiv(-delta - inner, g.s[1]), Wide(1 - g.n[1]));
+      last = std::min(FloorDiv(inner - delta, g.s[1]) + 1, Wide(g.n[1] - 1));
+    }
+    for (; j <= last; ++j) {
+      const Wide off = delta + j * g.s[1];  // wanted: -width < off + i s < width, |i| < n
+      Wide i = 0;
+      if (g.n[0] > 1) i = std::min(std::max(FloorDiv(-g.width - off, g.s[0]) + 1, Wide(1 - g.n[0])), Wide(g.n[0] - 1));
+      if (off + i * g.s[0] > -g.width && off + i * g.s[0] < g.width) return true;
+    }
+    return false;
+  }
+  for (int64_t j = 0; j < x.n[1]; ++j)
+    for (int64_t i = 0; i < x.n[0]; ++i)
+      if (Meets(g, static_cast<uintptr_t>(Wide(x.base) + j * x.s[1] + i * x.s[0]), x.width)) return true;
+  return false;
+}
+
+struct Read {  // an array that a gradient's kernel reads
+  const void *p;
+  int64_t bytes;
+  const char *what;
+};
+
+// A gradient's rows must not lie over each other, nor over anything that other units read while they are written.
+// The logits themselves, element for element, will do: a unit has loaded its own before it stores, and nothing
+// that it loads of another's is used.
+int CheckGrad(const kd_frame_rows *r, void *dx, int64_t batch_stride, int64_t row_stride,
+              std::initializer_list<Read> reads, GradOut *o) {
   if (!dx) return SetError(KD_E_INVALID, "bad argument: grad is NULL");
   if (reinterpret_cast<uintptr_t>(dx) % ElemBytes(r->dtype))
     return SetError(KD_E_INVALID, "bad argument: grad is not aligned to its type");
-  int64_t n[2] = {r->steps, r->batch}, s[2] = {row_stride, batch_stride};
-  if (s[0] > s[1]) {
-    std::swap(n[0], n[1]);
-    std::swap(s[0], s[1]);
+  Region g(dx, r, batch_stride, row_stride), x(r->logits, r, r->batch_stride, r->row_stride);
+  if ((g.n[0] > 1 && g.s[0] < g.width) || (g.n[1] > 1 && g.s[1] < g.Inner()))
+    return SetError(KD_E_INVALID, "bad argument: the gradient's rows overlap");
+  if (!g.Same(x)) {
+    g.Merge();
+    x.Merge();
+    if (Meets(g, x))
+      return SetError(KD_E_INVALID, "bad argument: the gradient lies across the logits (some memory location is another "
+                                    "element of theirs)");
   }
-  int64_t span = r->vocab;
-  for (int i = 0; i < 2; ++i) {
-    if (n[i] <= 1) continue;
-    if (s[i] < span) return SetError(KD_E_INVALID, "bad argument: the gradient's rows overlap");
-    span += (n[i] - 1) * s[i];
-  }
+  for (const Read &a : reads)
+    if (a.p && Meets(g, reinterpret_cast<uintptr_t>(a.p), a.bytes))
+      return SetError(KD_E_INVALID, std::string("bad argument: the gradient lies across ") + a.what);
   o->dx = dx;
   o->batch_stride = batch_stride;
   o->row_stride = row_stride;
@@ -1800,7 +1888,15 @@ int kd_token_scores_grad(const kd_frame_rows *rows, const void *tokens, int32_t 
       return SetError(KD_E_INVALID, "bad argument: token_bytes must be 4 or 8");
     if (!n) return KD_OK;
     if (!stats || (grad_entropy && !entropy)) return SetError(KD_E_INVALID, "bad argument: stats / entropy is NULL");
-    if (int rc = CheckGrad(rows, grad, grad_batch_stride, grad_row_stride, &a.o)) return rc;
+    if (int rc = CheckGrad(rows, grad, grad_batch_stride, grad_row_stride,
+                           {{rows->lengths, 4 * rows->batch, "lengths"},
+                            {tokens, n * token_bytes, "tokens"},
+                            {stats, n * 8, "stats"},
+                            {entropy, n * 4, "entropy"},
+                            {grad_logp, n * 4, "grad_logp"},
+                            {grad_entropy, n * 4, "grad_entropy"}},
+                           &a.o))
+      return rc;
     a.tokens = tokens;
     a.token64 = token_bytes == 8;
     a.stats = stats;
@@ -1849,9 +1945,19 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
     if (!teacher->ids || !teacher->logits) return SetError(KD_E_INVALID, "bad argument: the teacher's list is NULL");
     if (!loss && !grad) return SetError(KD_E_INVALID, "bad argument: neither loss nor gradient asked for");
     if (!loss && !stats) return SetError(KD_E_INVALID, "bad argument: a gradient alone needs the loss's stats");
-    if (grad)
-      if (int rc = CheckGrad(rows, grad, grad_batch_stride, grad_row_stride, &a.o)) return rc;
     const size_t need = known ? 0 : kd_distill_loss_workspace(rows, grad != nullptr);
+    if (grad)
+      if (int rc = CheckGrad(rows, grad, grad_batch_stride, grad_row_stride,
+                             {{rows->lengths, 4 * rows->batch, "lengths"},
+                              {teacher->ids, n * teacher->slots * teacher->id_bytes, "the teacher's ids"},
+                              {teacher->logits, n * teacher->slots * ElemBytes(teacher->dtype), "the teacher's logits"},
+                              {weights, n * 4, "weights"},
+                              {upstream, n * 4, "upstream"},
+                              {loss, n * 4, "loss"},
+                              {stats, n * 8, "stats"},
+                              {workspace, static_cast<int64_t>(need), "the workspace"}},
+                             &a.o))
+        return rc;
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
       return SetError(KD_E_INVALID, "bad argument: the workspace is too small (kd_distill_loss_workspace) or unaligned");
     a.ids = teacher->ids;

@@ -7,7 +7,6 @@
 // same row: 4.3), and 15 through ctypes.  With a gradient through autograd 35 us (a product of two
 // tensors and its gradient: 27), and 120.
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -127,10 +126,11 @@ Tensor GradOut(const OptTensor &out, const Tensor &x) {
                     "out must have the logits' shape, dtype and device");
   NoTangent(*out, "out");
   TORCH_CHECK_VALUE(out->stride(-1) == 1 || out->size(-1) == 1, "out needs unit stride over the last (V) dimension");
-  at::assert_no_partial_overlap(*out, x);  // (the logits themselves will do)
-  // (written in place: a graph that saved it must notice)
-  out->unsafeGetTensorImpl()->bump_version();
   return *out;
+}
+// (written in place: a graph that saved it must notice)
+void Written(const OptTensor &out) {
+  if (out && out->defined()) out->unsafeGetTensorImpl()->bump_version();
 }
 
 // [B, T] rows that follow each other evenly in every tensor concerned are handed over as one run: no
@@ -194,6 +194,7 @@ Tensor TokenScoresGrad(const Tensor &x, const OptTensor &tokens, const OptTensor
   Join(rows.r, &bs, rs);
   Check(kd_token_scores_grad(&rows.r, Ptr<void>(tok), tok.defined() ? IdBytes(tok) : 0, Ptr<float>(st), Ptr<float>(h),
                              Ptr<float>(gl), Ptr<float>(gh), dx.data_ptr(), bs, rs, Stream(x)));
+  Written(out);
   return dx;
 }
 
@@ -279,6 +280,7 @@ std::pair<Tensor, Tensor> Distill(const Tensor &x, const Tensor &ids, const Tens
   t.dtype = DtypeCode(u);
   Check(kd_distill_loss(&rows.r, &t, Ptr<float>(w), static_cast<float>(temperature), Ptr<float>(loss),
                         Ptr<float>(stats), Ptr<float>(up), Ptr<void>(dx), bs, rs, Ptr<void>(ws), bytes, Stream(x)));
+  Written(out);
   return {loss, dx};
 }
 

@@ -74,8 +74,8 @@ def token_scores(logits, tokens=None, top=0, lengths=None):
 def token_scores_grad(logits, scores, tokens=None, lengths=None, grad_logp=None, grad_entropy=None, out=None):
     """The gradient of the logits for upstream gradients of scores.logp and scores.entropy (float32,
     shape logits.shape[:-1]; None: 0), where `scores` = token_scores(logits, tokens, ..., lengths).
-    Written to `out` (the logits' shape and dtype, rows that do not overlap; `logits` itself will do) or to
-    a new tensor."""
+    Written to `out` (the logits' shape and dtype, rows that do not overlap, apart from everything that is
+    read; `logits` itself will do) or to a new tensor."""
     return _frames.token_scores_grad(logits, tokens, _tensors(logits, lengths), scores.stats, scores.entropy, grad_logp,
                                      grad_entropy, out)
 
@@ -96,7 +96,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=
 
 def distill_loss_and_grad(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, lengths=None, out=None):
     """(loss, gradient of loss.sum() in the logits): distill_loss and its backward pass in one call,
-    which reads rows of up to 64 KiB (many rows of up to 256 KiB) once.  The gradient goes to `out` (the logits' shape and dtype,
-    rows that do not overlap; `logits` itself will do) or to a new tensor."""
+    which reads rows of up to 64 KiB (many rows of up to 256 KiB) once.  The gradient goes to `out` (the
+    logits' shape and dtype, rows that do not overlap, apart from everything that is read; `logits` itself will
+    do) or to a new tensor."""
     return _frames.distill_loss_and_grad(logits, teacher_ids, teacher_logits, weights, temperature,
                                          _tensors(logits, lengths), out)

@@ -112,3 +112,39 @@ def test_forward_mode_derivatives_are_refused(frames):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
         assert torch.equal(frames.token_scores(dual(x).detach()).entropy, sc.entropy)
+
+
+def test_a_gradient_within_padded_tensors(frames):
+    """`out` in the storage of the logits or of another input: refused where an element would be in the
+    place of another that is read, right where it is not."""
+    for v in (40, 3000, 20000, 70000):
+        wide = torch.randn(2, 5, 2 * v + 3).cuda()
+        ids, u = torch.randint(0, v, (2, 4, 3)).cuda(), torch.randn(2, 4, 3).cuda()
+        x = wide[:, :4, :v]
+        tokens, up = ids[..., 0].contiguous(), torch.randn(2, 4).cuda()
+        sc = frames.token_scores(x, tokens)
+        before = wide.clone()
+        version = wide._version
+        for out in (wide[:, :4, 1:v + 1], wide[:, :4, v - 1:2 * v - 1], wide[:, 1:, :v], wide[:, 1:, v // 2:v // 2 + v],
+                    wide.flatten()[5:5 + 8 * v].view(2, 4, v)):
+            for call in (lambda: frames.distill_loss_and_grad(x, ids, u, out=out),
+                         lambda: frames.token_scores_grad(x, sc, tokens, None, up, up, out=out),
+                         lambda: frames.distill_loss_and_grad(x[0], ids[0], u[0], out=out[0])):
+                with pytest.raises(RuntimeError, match="across the logits"):
+                    call()
+        assert torch.equal(wide, before) and wide._version == version
+        loss, want = frames.distill_loss_and_grad(x.clone(), ids, u)
+        for out in (wide[:, :4, v:2 * v], wide[:, :4, v + 3:], wide[:, :4, :v]):  # (the last: the logits themselves)
+            loss2, got = frames.distill_loss_and_grad(x, ids, u, out=out)
+            assert torch.equal(got, want) and got.data_ptr() == out.data_ptr() and torch.equal(loss, loss2)
+            assert wide._version > version
+            assert torch.equal(wide[:, 4], before[:, 4])
+    # other inputs
+    u = torch.randn(3, 4, 8).cuda()
+    x, ids = torch.randn(3, 4, 8).cuda(), torch.arange(8).expand(3, 4, 8).cuda()
+    with pytest.raises(RuntimeError, match="across the teacher's logits"):
+        frames.distill_loss_and_grad(x, ids, u, out=u)
+    sc = frames.token_scores(x, ids[..., 0])
+    up = x.new_zeros(13)
+    with pytest.raises(RuntimeError, match="across grad_logp"):
+        frames.token_scores_grad(x[..., :1], sc, ids[..., 0], None, up[1:].view(3, 4), None, out=up[:12].view(3, 4, 1))
