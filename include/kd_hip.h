@@ -395,8 +395,8 @@ typedef struct kd_teacher_rows {
  *   loss[row] = weight sum_k q_k (log q_k - log p_{id_k})     (a q_k of 0 adds 0)
  *   grad_j    = weight upstream / temperature (p_j - sum_{k: id_k = j} q_k)
  * A slot of -inf counts as empty; NaN or +inf in a teacher's list: NaN at its columns, and a NaN loss.
- * `weights`, `upstream`: [rows] or NULL (1).  A row of weight 0 or without a filled slot is not
- * read: loss 0, gradient 0.  A teacher's token that the student has at -inf: loss +inf (a student
+ * `weights`, `upstream`: [rows] or NULL (1).  A row of weight 0 is not read, and one without a filled
+ * slot may hold anything: loss 0, gradient 0.  A teacher's token that the student has at -inf: loss +inf (a student
  * row of -inf alone: p = 0).  `grad` NULL: the loss alone.  `stats` ([rows][2], or NULL with a
  * loss): maximum and sum of the row, written with a loss; with `loss` NULL they are read, and the
  * call computes the gradient alone (the same inputs as the call that wrote them).  `grad` may be

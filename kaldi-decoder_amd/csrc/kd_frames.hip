@@ -705,6 +705,7 @@ struct ScoresArgs {
   int32_t *top_i;
   Partial *part;       // split rows: [rows][nseg], and [rows][nseg][k] alternatives
   uint64_t *part_top;
+  const float *weights;  // a loss's, [rows] or null: the statistics of rows of weight 0 are not wanted
 };
 
 __device__ inline int64_t IdAt(const void *ids, int32_t id64, size_t at) {
@@ -798,8 +799,9 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresK
   const Unit u = GetUnit(a.r, unit);
   if (u.skip) {
     if (!SPLIT) WriteRowNothing<TPU>(a, u.row, tid);
-    return;  // (split: the joining kernel writes, and reads no part of such a row)
+    return;  // (split: the joining kernel writes, and uses no part of such a row)
   }
+  if (SPLIT && !ENT && a.weights && a.weights[u.row] == 0.0f) return;  // (a loss's statistics: as well)
   const typename T::Store *x = RowPtr<T>(a.r.x, a.r.batch_stride, a.r.row_stride, u);
   U4 r[NCH];
   LoadUnit<T, NCH, TPU>(x + u.lo, u.n, tid, r);
@@ -1978,6 +1980,7 @@ int kd_distill_loss(const kd_frame_rows *rows, const kd_teacher_rows *teacher, c
       s.r = a.r;
       s.k2 = a.k2;
       s.part = static_cast<Partial *>(workspace);
+      s.weights = weights;
       if (!a.stats)
         a.stats = reinterpret_cast<float *>(static_cast<char *>(workspace) +
                                             Align(static_cast<size_t>(n) * p.nseg * sizeof(Partial)));

@@ -87,8 +87,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=
 
     `teacher_ids` (int32 or int64) and `teacher_logits` (float32, float16, bfloat16; log-probabilities
     serve as well) [..., K], K <= 256; an id outside [0, V), such as -1, or a logit of -inf marks an
-    empty slot, a token that is listed twice counts twice.  `weights` float32, shape logits.shape[:-1]: rows of weight 0, rows
-    without a listed token and rows behind `lengths` are not read (loss 0, gradient 0).  The loss
+    empty slot, a token that is listed twice counts twice.  `weights` float32, shape logits.shape[:-1]: rows
+    of weight 0 and rows behind `lengths` are not read, rows without a listed token may hold anything (loss
+    0, gradient 0).  The loss
     (float32, shape logits.shape[:-1]) is differentiable in the logits alone.  Where the weights are all
     that scales it (a mean: weights of 1 / rows), distill_loss_and_grad does the work of both passes in one."""
     return _frames.distill_loss(logits, teacher_ids, teacher_logits, weights, temperature, _tensors(logits, lengths))

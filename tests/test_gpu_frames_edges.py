@@ -1,5 +1,6 @@
 """kaldi_decoder.frames on the GPU at values, lengths and layouts that its documentation allows and that
 only unusual batches have; against the definition in 64 bits (frames_ref.py) where there is a value."""
+import ctypes as C
 
 import pytest
 import torch
@@ -148,3 +149,23 @@ def test_a_gradient_within_padded_tensors(frames):
     up = x.new_zeros(13)
     with pytest.raises(RuntimeError, match="across grad_logp"):
         frames.token_scores_grad(x[..., :1], sc, ids[..., 0], None, up[1:].view(3, 4), None, out=up[:12].view(3, 4, 1))
+
+
+def test_rows_of_weight_zero_are_not_read(frames):
+    """Long rows, cut into segments: those of weight 0 leave no partial results in the workspace."""
+    from kaldi_decoder import cabi
+    n, v = 16, 70000
+    x = torch.randn(n, v).cuda()
+    ids, u = torch.zeros(n, 1, dtype=torch.int32).cuda(), torch.zeros(n, 1).cuda()
+    w = (torch.arange(n) % 2).float().cuda()
+    loss = torch.empty(n).cuda()
+    rows = cabi.FrameRows(x.data_ptr(), 1, n, v, 0, v, None, 0, 0)
+    teacher = cabi.TeacherRows(ids.data_ptr(), u.data_ptr(), 1, 4, 0)
+    bytes_ = cabi.lib().kd_distill_loss_workspace(C.byref(rows), 0)
+    ws = torch.full((bytes_,), 0x5a, dtype=torch.uint8).cuda()
+    assert cabi.lib().kd_distill_loss(C.byref(rows), C.byref(teacher), w.data_ptr(), 1.0, loss.data_ptr(), None, None,
+                                      None, 0, 0, ws.data_ptr(), bytes_, torch.cuda.current_stream().cuda_stream) == 0
+    want = frames.distill_loss(x, ids, u)
+    assert torch.equal(loss, torch.where(w > 0, want, torch.zeros_like(want)))
+    part = ws[:bytes_ - 256].view(n, -1)  # (16 bytes a segment, all rows' first; then 8 bytes a row)
+    assert part[0::2].eq(0x5a).all() and part[1::2].ne(0x5a).any(-1).all()
