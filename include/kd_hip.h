@@ -345,8 +345,8 @@ int kd_batch_set_log_softmax(kd_batch *b, int32_t on);
  * stream, another captured graph) need one each.  Sums and statistics are f32; a call gives the same
  * bits from run to run (a row's last bits may depend on the number of rows it is called with: few
  * long rows are cut into more pieces).
- * vocab <= 2^24; a call has fewer than 2^32 threads, and a row takes 16 of them (up to 2 KiB), 64 (8 KiB),
- * 256 (32 KiB), 512 (64 KiB) or 256 for each 32 KiB: beyond that KD_E_INVALID, split the call. */
+ * vocab <= 2^24; a call has fewer than 2^32 threads in workgroups of 256 and more, and a row takes 16 of them (up to
+ * 2 KiB), 64 (8 KiB), 256 (32 KiB), 512 (64 KiB) or 256 for each 32 KiB: beyond that KD_E_INVALID, split the call. */
 #define KD_DTYPE_F32 0
 #define KD_DTYPE_F16 1
 #define KD_DTYPE_BF16 2

@@ -1602,6 +1602,11 @@ Plan MakePlan(int64_t vocab, int dtype, int64_t rows, Purpose what, int top, boo
   return p;
 }
 
+int64_t NumBlocks(int64_t units, const Plan &p) {
+  const int64_t per = std::max(kBlock / p.tpu, 1);
+  return (units + per - 1) / per;
+}
+
 int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64_t *rows, int top, bool narrow) {
   if (!r || r->batch < 0 || r->steps < 0) return SetError(KD_E_INVALID, "bad argument: rows");
   if (r->dtype != KD_DTYPE_F32 && r->dtype != KD_DTYPE_F16 && r->dtype != KD_DTYPE_BF16)
@@ -1612,8 +1617,8 @@ int CheckRows(const kd_frame_rows *r, Purpose what, Rows *out, Plan *plan, int64
     return SetError(KD_E_INVALID, "bad argument: more than 2^31 - 1 rows");
   *rows = r->batch * r->steps;
   *plan = MakePlan(r->vocab, r->dtype, *rows, what, top, narrow);
-  // (a grid has fewer than 2^32 threads)
-  if (*rows * plan->nseg > ((int64_t(1) << 32) - 1) / plan->tpu)
+  // (a grid has fewer than 2^32 threads, those of its last workgroup included)
+  if (NumBlocks(*rows * plan->nseg, *plan) * std::max(plan->tpu, kBlock) > (int64_t(1) << 32) - 1)
     return SetError(KD_E_INVALID, "bad argument: rows x vocab is too large for one call");
   if (r->batch_stride < 0 || r->row_stride < 0) return SetError(KD_E_INVALID, "bad argument: negative stride");
   if (*rows && !r->logits) return SetError(KD_E_INVALID, "bad argument: logits is NULL");
@@ -1742,8 +1747,7 @@ int CheckGrad(const kd_frame_rows *r, void *dx, int64_t batch_stride, int64_t ro
 }
 
 uint32_t Blocks(const Rows &r, const Plan &p) {
-  const uint64_t units = static_cast<uint64_t>(r.rows) * r.nseg, per = std::max(kBlock / p.tpu, 1);
-  return static_cast<uint32_t>((units + per - 1) / per);
+  return static_cast<uint32_t>(NumBlocks(static_cast<int64_t>(r.rows) * r.nseg, p));
 }
 
 // f(T{}, NCH, TPU as constants) for a plan.

@@ -127,3 +127,19 @@ def test_gradients_that_lie_across_other_inputs():
         args[i] = g + 316
         rc = cabi.lib().kd_token_scores_grad(C.byref(rows), args[0], 4, *args[1:], g, 40, 10, None)
         assert rc == -1 and b"across" in cabi.lib().kd_last_error(), i
+
+
+@pytest.mark.parametrize("vocab,most", [(4, 2 ** 28 - 16), (512, 2 ** 28 - 16), (2048, 2 ** 26 - 4), (8192, 2 ** 24 - 1)])
+def test_the_largest_grid(vocab, most):
+    """Rows of 16, 64 and 256 threads each: the last workgroup counts whole.  (Outputs that are missing end
+    the calls that are not too large.)"""
+    L, one = cabi.lib(), 4096
+    teacher = C.byref(cabi.TeacherRows(one, one, 3, 4, 0))
+    for rows, text in ((most, b""), (most + 1, b"too large")):
+        r = C.byref(cabi.FrameRows(one, 1, rows, vocab, 0, vocab, None, 0, 0))
+        for call, missing in (
+                (lambda: L.kd_token_scores(r, None, 0, 0, None, None, None, None, None, None, 0, None), b"output"),
+                (lambda: L.kd_token_scores_grad(r, None, 0, None, None, None, None, one, 0, vocab, None), b"stats"),
+                (lambda: L.kd_distill_loss(r, teacher, None, 1.0, None, None, None, None, 0, 0, None, 0, None),
+                 b"neither")):
+            assert call() == -1 and (text or missing) in L.kd_last_error(), (rows, L.kd_last_error())
