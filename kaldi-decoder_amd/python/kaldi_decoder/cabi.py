@@ -471,8 +471,10 @@ class Batch:
         logits they are the log_softmax of (any type frames.token_scores takes).  `tokens` int32 [B, T]:
         the column that each frame of the best path took -- LogLikelihood(frame, ilabel) reads column
         ilabel - 1 (csrc/decodable-ctc.cc:22-31) --, -1 behind its end; `scores`: frames.TokenScores of
-        them, with `top` alternatives a frame.  For batches that give best paths (not LatticeBatch: an
-        error, as best_paths is), decoded from frame 0 on."""
+        them, with `top` alternatives a frame.  An utterance without a path (`paths[i].ok` False: its
+        search died) has token -1 and logp -inf on every frame before its length, not the 0 of frames
+        behind the length.  For batches that give best paths (not LatticeBatch: an error, as
+        best_paths is), decoded from frame 0 on."""
         import torch
         from . import frames
         if logits.dim() != 3 or logits.shape[0] != self.batch:
@@ -483,9 +485,22 @@ class Batch:
             labels = path.isyms
             if len(labels) > logits.shape[1]:
                 raise ValueError(f"utterance {i}: a best path of {len(labels)} frames, logits of {logits.shape[1]}")
+            if len(labels) and labels.max() > logits.shape[2]:
+                raise ValueError(f"utterance {i}: a best path through column {labels.max() - 1}, logits of "
+                                 f"{logits.shape[2]} columns")
             tokens[i, :len(labels)] = labels - 1
         tokens = torch.from_numpy(tokens).to(logits.device)
-        return paths, tokens, frames.token_scores(logits, tokens, top=top, lengths=lengths)
+        scores = frames.token_scores(logits, tokens, top=top, lengths=lengths)
+        dead = [i for i, path in enumerate(paths) if not path.ok]
+        if dead:
+            rows = torch.zeros(logits.shape[:2], dtype=torch.bool)
+            rows[dead] = True
+            rows = rows.to(logits.device)
+            if lengths is not None:
+                rows &= torch.arange(logits.shape[1], device=logits.device) < torch.as_tensor(
+                    lengths, device=logits.device).unsqueeze(-1)
+            scores = scores._replace(logp=scores.logp.masked_fill(rows, float("-inf")))
+        return paths, tokens, scores
 
     def frame_tokens(self, utt, frame_plus_one):
         cnt = C.c_int32(0)

@@ -2,6 +2,7 @@
 import ctypes as C
 import random
 
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -143,3 +144,18 @@ def test_the_largest_grid(vocab, most):
                 (lambda: L.kd_distill_loss(r, teacher, None, 1.0, None, None, None, None, 0, 0, None, 0, None),
                  b"neither")):
             assert call() == -1 and (text or missing) in L.kd_last_error(), (rows, L.kd_last_error())
+
+
+def test_best_path_through_columns_that_the_logits_do_not_have():
+    class Decoded:  # (a batch of one utterance, decoded over wider rows)
+        batch = 1
+
+        def best_paths(self, use_final_probs):
+            il = np.array([2, 0, 5, 1], np.int32)
+            return [cabi.Path(True, il, il, il, np.zeros(4, np.float32), np.zeros(4, np.float32), (0.0, 0.0))]
+    with pytest.raises(ValueError, match="column 4"):
+        cabi.Batch.best_path_scores(Decoded(), torch.zeros(1, 3, 4))
+    with pytest.raises(ValueError, match="3 frames"):
+        cabi.Batch.best_path_scores(Decoded(), torch.zeros(1, 2, 9))
+    with pytest.raises(ValueError, match="CUDA tensor"):  # (five columns are enough: the next refusal)
+        cabi.Batch.best_path_scores(Decoded(), torch.zeros(1, 3, 5))

@@ -169,3 +169,28 @@ def test_rows_of_weight_zero_are_not_read(frames):
     assert torch.equal(loss, torch.where(w > 0, want, torch.zeros_like(want)))
     part = ws[:bytes_ - 256].view(n, -1)  # (16 bytes a segment, all rows' first; then 8 bytes a row)
     assert part[0::2].eq(0x5a).all() and part[1::2].ne(0x5a).any(-1).all()
+
+
+def test_scores_of_utterances_without_a_path(frames):
+    """An utterance whose search died scores -inf, not the 0 of a certain one; columns that the logits do
+    not have are an error."""
+    from kaldi_decoder import cabi, synth
+    # 0 -1-> 1 -2-> 2 (final), and no way on: a third frame leaves no token
+    g = synth.graph_from_arcs(3, 0, [(0, 1, 1, 1, 0.0), (1, 2, 2, 2, 0.0)], {2: 0.0})
+    x = torch.log_softmax(torch.randn(3, 4, 5, generator=torch.Generator().manual_seed(0)), -1).cuda()
+    for lengths in ([2, 3, 4], torch.tensor([2, 3, 4]).cuda(), torch.tensor([2, 3, 4], dtype=torch.int32)):
+        bt = cabi.Batch(cabi.Graph(g), max_batch=3, beam=100.0)
+        bt.decode_tensor(x, lengths)
+        paths, tokens, sc = bt.best_path_scores(x, lengths, top=2)
+        assert [p.ok for p in paths] == [True, False, False]
+        assert tokens[0].tolist() == [0, 1, -1, -1] and tokens[1:].eq(-1).all()
+        assert torch.isfinite(sc.logp[0]).all() and sc.logp[0, 2:].eq(0).all()
+        assert sc.logp[1].tolist() == [-INF, -INF, -INF, 0.0] and sc.logp[2].eq(-INF).all()
+        assert sc.entropy[1, :3].gt(0).all()
+    leaf = x.clone().requires_grad_()
+    sc = bt.best_path_scores(leaf)[2]
+    assert sc.logp[1:].eq(-INF).all()
+    sc.logp[0].sum().backward()
+    assert leaf.grad[1:].eq(0).all() and leaf.grad[0].ne(0).any()
+    with pytest.raises(ValueError, match="column"):
+        bt.best_path_scores(x[..., :1])
