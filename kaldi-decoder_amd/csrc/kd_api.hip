@@ -1333,7 +1333,12 @@ static int StageHost(kd_batch *b, const float *const *loglikes, int32_t num_cols
   KD_HIP_TRY(b->staging.Reserve(total));
   size_t pos = 0;
   for (int i = 0; i < b->batch; ++i) {
-    if (count[i]) {
+    // (rows without a gap are one plain copy: pitched copies from pageable memory have been seen to go row by
+    // row, 2.3 ms for a matrix of 250 x 500, where one copy takes 0.02)
+    if (count[i] && row_stride == num_cols) {
+      KD_HIP_TRY(hipMemcpyAsync(b->staging.p + pos, loglikes[i] + first[i] * row_stride,
+                                count[i] * num_cols * sizeof(float), hipMemcpyHostToDevice, b->stream));
+    } else if (count[i]) {
       KD_HIP_TRY(hipMemcpy2DAsync(b->staging.p + pos, num_cols * sizeof(float),
                                   loglikes[i] + first[i] * row_stride, row_stride * sizeof(float),
                                   num_cols * sizeof(float), count[i], hipMemcpyHostToDevice,
