@@ -91,6 +91,11 @@ def algorithmic_bytes(stats, V):
         max_tokens=int(stats[:, 8].max()), spill_frames=int(s[9])), (16 * a_scan + rest)
 
 
+def library_path():
+    return os.path.join(ROOT, "kaldi-decoder_amd", "python", "kaldi_decoder", "lib",
+                        os.environ.get("KD_HIP_LIB", "libkd_hip.so"))
+
+
 def profiled_traffic(workload_desc, utt_frames_per_launch, prune_interval, min_active=0):
     """HBM bytes per launch from the newest committed rocprofv3 PMC summary
     (profiles/rNN_summary.json, written by tools/summarize_profile.py from separate
@@ -98,8 +103,14 @@ def profiled_traffic(workload_desc, utt_frames_per_launch, prune_interval, min_a
     no summary for this workload and these options.  The counters are per launch: a
     summary taken on launches of another size (--steps-per-call) is scaled by the
     utterance-frames per launch, which is what the traffic is proportional to, and the
-    source says so."""
+    source says so, as it does where the summary is of another build of the library."""
     import glob
+    import hashlib
+    try:
+        with open(library_path(), "rb") as f:
+            here = hashlib.sha256(f.read()).hexdigest()[:16]
+    except OSError:
+        here = None
     best = None
     for path in sorted(glob.glob(os.path.join(ROOT, "profiles", "r*_summary.json"))):
         try:
@@ -121,6 +132,9 @@ def profiled_traffic(workload_desc, utt_frames_per_launch, prune_interval, min_a
                     f"{src} (measured on launches of {theirs} utterance-frames, scaled to {utt_frames_per_launch})")
         else:
             best = (d["hbm_bytes_per_launch"], src)
+        theirs = d.get("library_sha256")
+        if theirs and here and theirs != here:
+            best = (best[0], f"{best[1]}, of library {theirs}; this one is {here}")
     return best
 
 
