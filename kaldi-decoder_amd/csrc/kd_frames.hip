@@ -132,11 +132,13 @@ __device__ inline const typename T::Store *RowPtr(const void *x, int64_t batch_s
 template <int TPU>
 constexpr int kThreads = TPU < kBlock ? kBlock : TPU;  // of a workgroup
 // Waves a SIMD that a kernel is compiled for (1: as many as its registers allow).  Units of 512 lanes
-// take two a SIMD, so 68 registers instead of 64 would cost one unit in four (40.4 instead of 43.2 us
+// take two a SIMD, so 68 registers instead of 64 would cost one unit in four (38.0 instead of 42.0 us
 // for 2048 rows of 32768 bf16 with 64 alternatives); units of 16 lanes hold 16 addresses a lane unless
-// told not to (24.7 instead of 25.6 us for the loss and gradient of 24000 rows of 500 with 32 slots).
-template <int TPU, int NCH>
-constexpr int kOccupancy = TPU == 16 || TPU == 512 || (TPU == 1024 && NCH <= 8) ? 8 : 1;
+// told not to (18.4 instead of 18.6 us for the loss and gradient of 24000 rows of 500 with 8 slots), but
+// with four slots a lane loss and gradient together would spill registers (32 slots: 27.1 us, and 25.1 left
+// alone).  SN: slots a lane, of such a kernel.
+template <int TPU, int NCH, int SN = 1>
+constexpr int kOccupancy = (TPU == 16 && SN == 1) || TPU == 512 || (TPU == 1024 && NCH <= 8) ? 8 : 1;
 template <int TPU>
 __device__ inline int UnitLane() {
   return TPU < kBlock ? (threadIdx.x & (TPU - 1)) : threadIdx.x;
@@ -1393,7 +1395,7 @@ __device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU, 
 // in two kernels, three passes over memory, take 628.  (A row of 256 KiB fills half a CU's registers, so
 // its loads, sums and stores do not overlap with another's on the same CU; other CUs' do.)
 template <class T, int NCH, int TPU, int SN, bool GRAD>
-__global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void DistillKernel(const DistillArgs a) {
+__global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH, GRAD ? SN : 1>)) void DistillKernel(const DistillArgs a) {
   __shared__ TeacherList<TPU, SN> lists[kUnits<TPU>];
   const int tid = UnitLane<TPU>();
   const uint32_t unit = UnitNumber<TPU>();
