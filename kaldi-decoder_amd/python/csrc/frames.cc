@@ -125,6 +125,8 @@ Tensor GradOut(const OptTensor &out, const Tensor &x) {
   TORCH_CHECK_VALUE(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->device() == x.device(),
                     "out must have the logits' shape, dtype and device");
   NoTangent(*out, "out");
+  TORCH_CHECK(!out->is_inference() || c10::InferenceMode::is_enabled(),
+              "out is an inference tensor: it can be written in inference mode alone");
   TORCH_CHECK_VALUE(out->stride(-1) == 1 || out->size(-1) == 1, "out needs unit stride over the last (V) dimension");
   return *out;
 }

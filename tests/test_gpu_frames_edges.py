@@ -194,3 +194,22 @@ def test_scores_of_utterances_without_a_path(frames):
     assert leaf.grad[1:].eq(0).all() and leaf.grad[0].ne(0).any()
     with pytest.raises(ValueError, match="column"):
         bt.best_path_scores(x[..., :1])
+
+
+def test_inference_tensors(frames):
+    """`out` made in inference mode is written there and, outside of it, refused before anything is."""
+    x, ids, u = torch.randn(3, 40).cuda(), torch.arange(2).expand(3, 2).cuda(), torch.randn(3, 2).cuda()
+    loss, want = frames.distill_loss_and_grad(x, ids, u)
+    with torch.inference_mode():
+        out = torch.zeros(3, 40).cuda()
+        loss2, got = frames.distill_loss_and_grad(x, ids, u, out=out)
+        assert torch.equal(got, want) and torch.equal(loss, loss2) and torch.equal(out, want)
+        sc = frames.token_scores(x, ids[:, 0], top=3)
+        out.zero_()
+    assert torch.equal(sc.logp, frames.token_scores(x, ids[:, 0]).logp)
+    with pytest.raises(RuntimeError, match="inference"):
+        frames.distill_loss_and_grad(x, ids, u, out=out)
+    with pytest.raises(RuntimeError, match="inference"):
+        frames.token_scores_grad(x, sc, ids[:, 0], None, loss, None, out=out)
+    torch.cuda.synchronize()
+    assert out.eq(0).all()
