@@ -335,8 +335,8 @@ int kd_batch_set_log_softmax(kd_batch *b, int32_t on);
  *
  * Rows: [batch][steps][vocab] logits (unit stride over the vocabulary, any non-negative strides,
  * in elements, over the others; 2-D logits are batch = 1).  `lengths` (device, [batch], or NULL):
- * rows at or behind their utterance's length are not read, their outputs are 0 (alternatives
- * -1 / -inf) and so are their gradients.  Arrays of one value a row are contiguous [batch][steps].
+ * rows at or behind their utterance's length (beyond the steps: none; below 0: all) are not read, their
+ * outputs are 0 (alternatives -1 / -inf) and so are their gradients.  Arrays of one value a row are contiguous [batch][steps].
  *
  * All pointers are device pointers on `device`.  A call enqueues on `stream` (a hipStream_t, NULL =
  * default) and returns: no allocation, no synchronisation, no state of the library's, so calls may

@@ -611,9 +611,12 @@ __device__ __noinline__ uint64_t KthElement(const SRC src, int *red, float floor
   return Key(val, col);
 }
 
-// (What alternatives cost beside the statistics, 2048 rows of 32768 bf16: 24 us with none, 28 with 1,
-// 31 with 32, 36 with 64; a single row of 262144: 4.9 us with none, 9.3 with 20, most of it the steps that
-// wait for each other in the two kernels.)
+// (What alternatives cost beside the statistics, 2048 rows of 32768 bf16: 28 us with none, 31 with 1,
+// 33 with 32, 38 with 64; a single row of 262144: 4.8 us with none, 9.6 with 20, most of it the steps that
+// wait for each other in the two kernels.  The bisection reads a unit up to 57 times, with two barriers each
+// time: constant rows, or rows where fewer than k columns are left above a mask of one finite value -- mask
+// with -inf -- take 15 to 60 times as long: 32000 x 500 f32 with 8 alternatives 544 instead of 16.6 us, 64 x
+// 131072 bf16 with 20 545 instead of 12.8, 2048 x 32768 bf16 with 64 2165 instead of 35.8.)
 //
 // Puts the unit's K largest elements in order and hands (place, key) to `out`, once per place from
 // some lane; places without an element get key 0.  `threshold`: at least k of the unit's elements
@@ -789,8 +792,9 @@ __device__ inline void WriteNoTop(float *v, int32_t *i, float val, int k, int ti
 
 // Statistics, scores and alternatives of a unit: an element costs 1.5 operations for the maximum
 // (v_maximum3 takes two, f16 and bf16 are unpacked first) and 7 (fma, exp2 -- a quarter of the rate --,
-// two sums and their guard), so rows of bf16 keep the vector units as busy as the memory: 268 M elements
-// take 128 us, 4.2 TB/s, where a plain sum over the same bytes by the library runs at 4.0.
+// two sums and their guard), so rows of bf16 keep the vector units busy for 66 % of a pass's cycles (87 % with
+// 64 alternatives; profiles/frames_counters.csv): 268 M elements take 128 us, 4.2 TB/s, where a plain sum over the
+// same bytes by the library runs at 4.0.
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
 __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresKernel(const ScoresArgs a) {
   __shared__ Scratch<TPU> scratch[TOP || TPU > 64 ? kUnits<TPU> : 1];
@@ -974,8 +978,8 @@ __global__ __launch_bounds__(kBlock) void ScoresJoinKernel(const ScoresArgs a) {
 // ---- scores of short rows --------------------------------------------------------------------
 // Rows of up to 2 KiB: a wave takes four, 16 lanes (one DPP row) each.  What such a row costs is not
 // its bytes but the steps that are taken once a row -- reductions, threshold, ranking --, and these
-// serve four rows here: 24000 rows of 500 f32 with 8 alternatives 12.8 us (9.5 without), and 19.5 with a
-// wave a row.  More than 16 alternatives need the 64 groups of a whole wave (21.5 us with 17).
+// serve four rows here: 24000 rows of 500 f32 with 8 alternatives 14.5 us (10.5 without), and 21.4 (12.4)
+// with a wave a row.  More than 16 alternatives need the 64 groups of a whole wave (21.0 us with 17).
 
 // The k-th largest (k <= 16) of 16 lanes' pairs, in all lanes.
 __device__ inline float RowKthLargest(float a, float b, int k) {
@@ -1391,8 +1395,8 @@ __device__ inline void LoadAtSlots(const typename T::Store *x, const Slots<TPU, 
 }
 
 // Whole rows: loss, and with GRAD the gradient from the registers that the statistics were taken of:
-// 4096 rows of 131072 bf16 in 467 us, 4.6 TB/s of one read and one write, where statistics and gradient
-// in two kernels, three passes over memory, take 628.  (A row of 256 KiB fills half a CU's registers, so
+// 4096 rows of 131072 bf16 in 470 us, 4.6 TB/s of one read and one write, where statistics and gradient
+// in two kernels, three passes over memory, take 622.  (A row of 256 KiB fills half a CU's registers, so
 // its loads, sums and stores do not overlap with another's on the same CU; other CUs' do.)
 template <class T, int NCH, int TPU, int SN, bool GRAD>
 __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH, GRAD ? SN : 1>)) void DistillKernel(const DistillArgs a) {
@@ -1563,14 +1567,14 @@ int Launch(void (*kernel)(ARGS), uint32_t blocks, const ARGS &args, void *stream
 int64_t ElemBytes(int dtype) { return dtype == KD_DTYPE_F32 ? 4 : 2; }
 
 // How rows are dealt out: TPU lanes a unit, up to NCH 16-byte loads each.  Both sides of each rule, in
-// us (D: loss and gradient of bf16 rows; S: scores with 20 alternatives):
-//   whole to 64 KiB         S 1 x 32768 7.1, in segments 10.6; D 8 x 32768 10.3 and 12.7; D 4096 x 32768
-//                           116 and 184
-//   1024 lanes, 128 KiB     D 64 x 65536 15.5, in segments 17.5; 16 x 65536 13.7 and 13.3; 4096 x 65536 219 and 338
-//   1024 lanes, 256 KiB     D 256 x 131072 33.5, in segments 44; 128 x 131072 26.8 and 27.4; 64: 24 and 21.5
+// us (D: loss and gradient of bf16 rows with 64 slots; S: scores with 20 alternatives):
+//   whole to 64 KiB         S 1 x 32768 7.2, in segments 9.2; D 8 x 32768 8.6 and 10.6; D 4096 x 32768
+//                           115 and 176
+//   1024 lanes, 128 KiB     D 64 x 65536 13.3, in segments 15.3; 16 x 65536 12.0 and 11.2; 4096 x 65536 219 and 334
+//   1024 lanes, 256 KiB     D 256 x 131072 32.2, in segments 43.1; 128 x 131072 25.1 and 25.2; 64: 22.4 and 19.5
 //                           (values alone are read once either way: 512 x 131072 41.7 and 29.4)
-//   smaller segments for    S 8 x 131072 9.9 with 256 units and more, 10.6 with 64; D 8 x 131072 13.3 and 14.8; S 1 x
-//   few rows                262144 9.3 and 9.4 (from 1024 units on the joining kernel's share grows: 16 x 131072
+//   smaller segments for    S 8 x 131072 9.8 with 256 units and more, 10.7 with 64; D 8 x 131072 11.2 and 12.5; S 1 x
+//   few rows                262144 9.6 and 10.3 (from 1024 units on the joining kernel's share grows: 16 x 131072
 //                           10.1 with 512, 10.8 with 1024).  That kernel holds at most kHeld x 256
 //                           alternatives in registers (1 x 262144 with 64: 14.1 with 32 units, 18.9 with 64)
 struct Plan {

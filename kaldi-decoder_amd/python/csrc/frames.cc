@@ -4,8 +4,8 @@
 //
 // Host C++ only.  The smallest of these calls take the GPU 4 us, so what a call does on the host is
 // what it costs: checks, three to five allocations and one C call are 4 to 6.5 us here (torch.neg of the
-// same row: 4.3), and 15 through ctypes.  With a gradient through autograd 35 us (a product of two
-// tensors and its gradient: 27), and 120.
+// same row: 4.2), and 15 through ctypes.  With a gradient through autograd 29 or 48 us, from process to
+// process, most of it torch's engine (a product of two tensors and its gradient: 27 or 45), and 120.
 
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
