@@ -333,16 +333,36 @@ __device__ inline int Popc(uint64_t m) { return __popcll(m); }
 // type's lowest value) any column that differs from m at all is 2^64 times smaller: there a power
 // of two stands in for k2 that makes m k2 exact, about 2^40, and such columns' e 0.
 // (1.5e-6 <= k2 <= 1.5e6, the range of the temperature.)
+// The maximum's own e comes out as `one`, 2^delta rounded, the same bits wherever it is computed.  What is
+// known to be 1 is therefore divided by it and not multiplied by another rounding of 2^-delta: a row that one
+// token has nearly to itself would lose two roundings of 1 in s, and so in its log p and 1 - p.
 struct Exponent {
-  float k2, c, delta;
+  float k2, c, delta, one;
   __device__ Exponent(float base, float k2_) {
     const bool far = !(fabsf(base * k2_) < 0x1p30f) && base != INFINITY;
     k2 = far ? __uint_as_float(__float_as_uint(0x1p40f / fabsf(base)) & 0x7f800000u) : k2_;
     c = base * k2;
     delta = fmaf(base, k2, -c);  // exponents come out larger by this much
+    one = __builtin_amdgcn_exp2f(delta);
+  }
+  __device__ float PerOne() const {  // 1 / one, within one step
+    const float r = __builtin_amdgcn_rcpf(one);
+    return fmaf(fmaf(-one, r, 1.0f), r, r);
   }
   __device__ float operator()(float x) const { return fmaf(x, k2, -c); }
 };
+
+// f(FIRST) + ... + f(FIRST + N - 1), in pairs: the 1 that a row's maximum brings in then takes part in a few
+// additions of a lane's and not in all that follow it, each of which would round it.
+template <int N, int FIRST = 0, class F>
+__device__ inline float PairSum(const F &f) {
+  if constexpr (N == 1) {
+    return f(FIRST);
+  } else {
+    const float a = PairSum<N / 2, FIRST>(f);
+    return a + PairSum<N / 2, FIRST + N / 2>(f);
+  }
+}
 
 // ---- the K largest -------------------------------------------------------------------------------
 // Order: larger value first, then lower column.  -inf and NaN are no candidates.
@@ -736,15 +756,13 @@ __device__ inline float Base(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ inline float LogSum(float s0) { return s0 == 0.0f ? 0.0f : logf(s0); }
 
 // A unit's s0 and s1 = sum e_j log2(e_j) without what the rounding of the exponents' c added to them
-// (Exponent).  The maximum's own e is exp2(delta) exp2(-delta), 1 but for two roundings: with a finite
-// maximum the sum is at least 1 and s1 at most 0, or a row that one token has to itself would give
-// log-probabilities above 0 and entropies below.  (NaN stays.)
-__device__ inline float Corrected0(float s0, float less, float m) {
-  s0 *= less;
-  return m == -INFINITY ? s0 : Max(s0, 1.0f);
+// (Exponent).  With a finite maximum the sum is 1 for it and what the others add, so at least 1, and s1 at most 0:
+// no log-probability above 0, no entropy below.  (NaN stays.)
+__device__ inline float Corrected0(float s0, const Exponent &e, float m) {
+  return m == -INFINITY ? s0 : fmaf(s0 - e.one, e.PerOne(), 1.0f);
 }
-__device__ inline float Corrected1(float s0, float s1, float delta, float less) {
-  return Min(fmaf(-delta, s0, s1) * less, 0.0f);
+__device__ inline float Corrected1(float s0, float s1, const Exponent &e) {
+  return Min(fmaf(-e.delta, s0, s1) * e.PerOne(), 0.0f);
 }
 
 // H = log s - ln 2 s1 / s, two terms that are at least 0.  (What cancels is within s1: delta s0, where delta is
@@ -838,13 +856,12 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresK
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     if (!Used<T, TPU>(c, u.n)) continue;
-#pragma unroll
-    for (int j = 0; j < T::kVec; ++j) {
+    s0 += PairSum<T::kVec>([&](int j) {
       const float t = exponent(T::Get(r[c], j)), e = __builtin_amdgcn_exp2f(t);
-      s0 += e;
       // (t is -inf for a masked column: 0 * -inf would be NaN)
       if (ENT) s1 = fmaf(e, fmaxf(t, kLowest), s1);
-    }
+      return e;
+    });
   }
   s0 = WaveSum(s0);
   if (ENT) s1 = WaveSum(s1);
@@ -857,9 +874,8 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresK
     s0 = SumOf<TPU>(s.red[1]);
     if (ENT) s1 = SumOf<TPU>(s.red[2]);
   }
-  const float less = __builtin_amdgcn_exp2f(-exponent.delta);
-  if (ENT) s1 = Corrected1(s0, s1, exponent.delta, less);
-  s0 = Corrected0(s0, less, m);
+  if (ENT) s1 = Corrected1(s0, s1, exponent);
+  s0 = Corrected0(s0, exponent, m);
 
   if (SPLIT) {
     if (tid == 0) a.part[unit] = Partial{m, s0, s1, 0.0f};
@@ -1060,18 +1076,17 @@ __global__ __launch_bounds__(kBlock) void ScoresShortKernel(const ScoresArgs a) 
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     if (!Used<T, 16>(c, n)) continue;
-#pragma unroll
-    for (int j = 0; j < T::kVec; ++j) {
-      const float t = exponent(T::Get(r[c], j)), e = __builtin_amdgcn_exp2f(t);
-      s0 += e;
+    const U4 v = r[c];  // (the array itself, caught by reference, would stay in memory)
+    s0 += PairSum<T::kVec>([&](int j) {
+      const float t = exponent(T::Get(v, j)), e = __builtin_amdgcn_exp2f(t);
       s1 = fmaf(e, fmaxf(t, kLowest), s1);
-    }
+      return e;
+    });
   }
   s0 = RowSum(s0);
   s1 = RowSum(s1);
-  const float less = __builtin_amdgcn_exp2f(-exponent.delta);
-  s1 = Corrected1(s0, s1, exponent.delta, less);
-  s0 = Corrected0(s0, less, m);
+  s1 = Corrected1(s0, s1, exponent);
+  s0 = Corrected0(s0, exponent, m);
   const float ls = LogSum(s0);
   if (l == 0) WriteRowScores(a, row, tok, m, s0, s1);
   if (!TOP) return;
@@ -1217,7 +1232,7 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH>)) void ScoresG
   const float gh = a.g_entropy ? a.g_entropy[u.row] : 0.0f;
   const int at = tok < 0 ? -T::kVec : static_cast<int>(tok) - u.lo;  // (may be outside the unit)
   const Exponent exponent(m, kLog2e);
-  const float inv = __builtin_amdgcn_exp2f(-exponent.delta) / s0, ls = logf(s0);
+  const float inv = 1.0f / (exponent.one * s0), ls = logf(s0);
   const float B = -kLn2 * gh * inv;
   const float A = (a.g_entropy ? -gl - gh * (a.entropy[u.row] - ls) : -gl) * inv - B * exponent.delta;
   StoreUnit<T, NCH, TPU>(dx, u.n, tid, r, [=](const U4 &v, int first, float *g) {
@@ -1360,7 +1375,7 @@ __device__ inline void WriteDistillGrad(const DistillArgs &a, const Unit &u, con
       const_cast<typename T::Store *>(RowPtr<T>(a.o.dx, a.o.batch_stride, a.o.row_stride, u)) + u.lo;
   const Exponent exponent(Base(m), a.k2);
   // (a student without a finite logit gives nothing any probability)
-  const float inv = s0 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-exponent.delta) / s0, scale = coef * inv;
+  const float inv = s0 == 0.0f ? 0.0f : 1.0f / (exponent.one * s0), scale = coef * inv;
   StoreUnit<T, NCH, TPU>(dx, u.n, tid, r, [=](const U4 &v, int, float *g) {
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) g[j] = scale * __builtin_amdgcn_exp2f(exponent(T::Get(v, j)));
@@ -1442,10 +1457,9 @@ __global__ __launch_bounds__(kThreads<TPU>, (kOccupancy<TPU, NCH, GRAD ? SN : 1>
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     if (!Used<T, TPU>(c, u.n)) continue;
-#pragma unroll
-    for (int j = 0; j < T::kVec; ++j) s0 += __builtin_amdgcn_exp2f(exponent(T::Get(r[c], j)));
+    s0 += PairSum<T::kVec>([&](int j) { return __builtin_amdgcn_exp2f(exponent(T::Get(r[c], j))); });
   }
-  s0 = Corrected0(UnitSum<TPU>(s0, list.red[3]), __builtin_amdgcn_exp2f(-exponent.delta), m);
+  s0 = Corrected0(UnitSum<TPU>(s0, list.red[3]), exponent, m);
   const float ls = LogSum(s0);
   const float loss = Divergence<TPU, SN>(a, t, xs, m, ls, w, list.red[4]);
   if (tid == 0) {
