@@ -810,7 +810,7 @@ __device__ inline void WriteNoTop(float *v, int32_t *i, float val, int k, int ti
 
 // Statistics, scores and alternatives of a unit: an element costs 1.5 operations for the maximum
 // (v_maximum3 takes two, f16 and bf16 are unpacked first) and 7 (fma, exp2 -- a quarter of the rate --,
-// two sums and their guard), so rows of bf16 keep the vector units busy for 66 % of a pass's cycles (87 % with
+// two sums and their guard), so rows of bf16 keep the vector units busy for 62 % of a pass's cycles (86 % with
 // 64 alternatives; profiles/frames_counters.csv): 268 M elements take 128 us, 4.2 TB/s, where a plain sum over the
 // same bytes by the library runs at 4.0.
 template <class T, int NCH, int TPU, bool SPLIT, bool ENT, bool TOP>
