@@ -336,7 +336,8 @@ int kd_batch_set_log_softmax(kd_batch *b, int32_t on);
  * Rows: [batch][steps][vocab] logits (unit stride over the vocabulary, any non-negative strides,
  * in elements, over the others; 2-D logits are batch = 1).  `lengths` (device, [batch], or NULL):
  * rows at or behind their utterance's length (beyond the steps: none; below 0: all) are not read, their
- * outputs are 0 (alternatives -1 / -inf) and so are their gradients.  Arrays of one value a row are contiguous [batch][steps].
+ * outputs are 0 (alternatives -1 / -inf) and so are their gradients.  Arrays of one value a row are
+ * contiguous [batch][steps].
  *
  * All pointers are device pointers on `device`.  A call enqueues on `stream` (a hipStream_t, NULL =
  * default) and returns: no allocation, no synchronisation, no state of the library's, so calls may
@@ -345,8 +346,9 @@ int kd_batch_set_log_softmax(kd_batch *b, int32_t on);
  * stream, another captured graph) need one each.  Sums and statistics are f32; a call gives the same
  * bits from run to run (a row's last bits may depend on the number of rows it is called with: few
  * long rows are cut into more pieces).
- * vocab <= 2^24; a call has fewer than 2^32 threads in workgroups of 256 and more, and a row takes 16 of them (up to
- * 2 KiB), 64 (8 KiB), 256 (32 KiB), 512 (64 KiB) or 256 for each 32 KiB: beyond that KD_E_INVALID, split the call. */
+ * vocab <= 2^24; a call has fewer than 2^32 threads in workgroups of 256 and more, and a row takes 16 of
+ * them (up to 2 KiB), 64 (8 KiB), 256 (32 KiB), 512 (64 KiB) or 256 for each 32 KiB: beyond that KD_E_INVALID,
+ * split the call. */
 #define KD_DTYPE_F32 0
 #define KD_DTYPE_F16 1
 #define KD_DTYPE_BF16 2

@@ -1688,9 +1688,6 @@ struct Region {
   }
   Wide Inner() const { return width + (n[0] - 1) * s[0]; }  // of a group
   Wide Span() const { return Inner() + (n[1] - 1) * s[1]; }
-  bool Same(const Region &o) const {
-    return base == o.base && n[0] == o.n[0] && n[1] == o.n[1] && s[0] == o.s[0] && s[1] == o.s[1] && width == o.width;
-  }
 };
 Wide FloorDiv(Wide a, Wide b) { return a / b - (a % b < 0); }  // (b > 0)
 // First and last of the 0 <= i < n with lo < i * s + width and i * s < hi; none: first > last.
@@ -1750,9 +1747,12 @@ int CheckGrad(const kd_frame_rows *r, void *dx, int64_t batch_stride, int64_t ro
   Region g(dx, r, batch_stride, row_stride), x(r->logits, r, r->batch_stride, r->row_stride);
   if ((g.n[0] > 1 && g.s[0] < g.width) || (g.n[1] > 1 && g.s[1] < g.Inner()))
     return SetError(KD_E_INVALID, "bad argument: the gradient's rows overlap");
-  if (!g.Same(x)) {
-    g.Merge();
-    x.Merge();
+  g.Merge();
+  x.Merge();
+  // (each row in its own logits' place: regions that are alike may have their dimensions the other way round)
+  const bool itself = dx == r->logits && (r->batch <= 1 || batch_stride == r->batch_stride) &&
+                      (r->steps <= 1 || row_stride == r->row_stride);
+  if (!itself) {
     if (Meets(g, x))
       return SetError(KD_E_INVALID, "bad argument: the gradient lies across the logits (some memory location is another "
                                     "element of theirs)");

@@ -8,15 +8,17 @@ teacher's rows gives -- differentiable, or as loss and gradient in one call
 
 Rows are a CUDA tensor [N, V] or [B, T, V], float32, float16 or bfloat16, with unit stride over V
 and any strides over the others (views of padded tensors are read in place); `lengths` [B] are the
-valid rows of each utterance, 0 to T as in `Batch.decode_tensor` (not checked here: they may be on the
-GPU): what lies behind is not read, scores 0 and gets gradient 0.  Sums are float32 whatever the rows' type.  Calls run on the current stream of
-the tensors' device, allocate through torch's allocator and do not synchronise (but for `lengths`
-that are not on the device yet): they can be captured into a graph.  A backward pass through
-autograd that is to be captured needs its leaves to have no live graph from outside the capture, as
-any of torch's; `token_scores_grad` and `distill_loss_and_grad` have no such condition.
+valid rows of each utterance, 0 to T as in `Batch.decode_tensor` (not checked here: they may be on
+the GPU): what lies behind is not read, scores 0 and gets gradient 0.  Sums are float32 whatever the
+rows' type.  Calls run on the current stream of the tensors' device, allocate through torch's
+allocator and do not synchronise (but for `lengths` that are not on the device yet): they can be
+captured into a graph.  A backward pass through autograd that is to be captured needs its leaves to
+have no live graph from outside the capture, as any of torch's; `token_scores_grad` and
+`distill_loss_and_grad` have no such condition.
 
-What is differentiable is so once, backwards: a second derivative (create_graph) and forward mode (a tensor that
-carries a tangent) raise an error.  `token_scores_grad` and `distill_loss_and_grad` are outside autograd altogether.
+What is differentiable is so once, backwards: a second derivative (create_graph) and forward mode (a
+tensor that carries a tangent) raise an error.  `token_scores_grad` and `distill_loss_and_grad` are
+outside autograd altogether.
 
 (The reference leaves all of this to its callers; its DecodableCtc takes log-probabilities,
 csrc/decodable-ctc.cc:28.)

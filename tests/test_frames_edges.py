@@ -159,3 +159,14 @@ def test_best_path_through_columns_that_the_logits_do_not_have():
         cabi.Batch.best_path_scores(Decoded(), torch.zeros(1, 2, 9))
     with pytest.raises(ValueError, match="CUDA tensor"):  # (five columns are enough: the next refusal)
         cabi.Batch.best_path_scores(Decoded(), torch.zeros(1, 3, 5))
+
+
+def test_a_gradient_over_the_transposed_logits():
+    """As many steps as utterances: the same places, but each row's another row's."""
+    at = 1 << 40
+    for n in (2, 3):
+        for a, b in (((n * V, V), (V, n * V)), ((V, n * V), (n * V, V)), ((V + 8, 5 * (V + 8)), (5 * (V + 8), V + 8))):
+            assert "across the logits" in _place(at, at, n, n, a, b)
+            assert not _place(at, at, n, n, a, a) and not _place(at, at, n, n, b, b)
+    assert not _place(at, at, 1, 1, (V, 3 * V), (3 * V, V))
+    assert not _place(at, at, 4, 1, (V, 9), (V, 7)) and not _place(at, at, 1, 4, (9, V), (7, V))

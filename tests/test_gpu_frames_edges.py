@@ -234,3 +234,19 @@ def test_precision_of_peaked_rows(frames, v):
     assert lp.min() > -0.5  # (the rows are what they are meant to be)
     off = (sc.logp.cpu().double() - lp).abs().mean().item()
     assert off <= ((3 + 8 + 6 + 3 + 1 + 1) / 3) ** 0.5 * 2 ** -24, off * 2 ** 24
+
+
+def test_a_gradient_over_the_transposed_logits(frames):
+    """As many steps as utterances: `out` = the logits' transpose is the same memory in another order."""
+    x = torch.randn(4, 4, 300).cuda()
+    ids, u = torch.zeros(4, 4, 2, dtype=torch.int32).cuda(), torch.randn(4, 4, 2).cuda()
+    before = x.clone()
+    with pytest.raises(RuntimeError, match="across the logits"):
+        frames.distill_loss_and_grad(x, ids, u, out=x.transpose(0, 1))
+    with pytest.raises(RuntimeError, match="across the logits"):
+        frames.token_scores_grad(x.transpose(0, 1), frames.token_scores(x), None, None, None, u[..., 0].contiguous(), out=x)
+    assert torch.equal(x, before)
+    _, want = frames.distill_loss_and_grad(before, ids, u)
+    t = x.transpose(0, 1)
+    _, got = frames.distill_loss_and_grad(t, ids.transpose(0, 1), u.transpose(0, 1), out=t)
+    assert torch.equal(x, want)
